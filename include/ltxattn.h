@@ -313,6 +313,178 @@ typedef struct ltxattn_rope_args {
  * MLX tensor times a bf16 table. */
 LTXATTN_API int ltxattn_rope(const ltxattn_rope_args* args, void* stream);
 
+/* ---- rotary positions ------------------------------------------------------ */
+
+/* Which elements of a head turn together.  With n = rotary_dim / 2 pairs, pair
+ * j is (x[j], x[j + n]) in the half layout and (x[2j], x[2j + 1]) in the
+ * interleaved one; elements from rotary_dim on are not turned. */
+typedef enum ltxattn_rotary_layout { LTXATTN_ROTARY_HALF = 0, LTXATTN_ROTARY_INTERLEAVED = 1 } ltxattn_rotary_layout;
+
+/* How the pair frequencies theta^(-j / n) are stretched for contexts longer
+ * than the trained one (n pairs, s = factor, L = trained_length).
+ *  - NONE: as they are.
+ *  - LINEAR: all divided by s.
+ *  - NTK: theta replaced by theta * s^(n / (n - 1)), which leaves pair 0 alone
+ *    and divides the slowest by s (a single pair: as they are).
+ *  - YARN: pairs that turn more than `fast` times in L stay, those that turn
+ *    less than `slow` times are divided by s, with a linear ramp over the pair
+ *    index between the two (rounded outwards to whole pairs); what is turned
+ *    is multiplied by 0.1 ln(s) + 1 (1 for s <= 1).
+ *  - BANDS: the same three bands with the ramp linear in the number of turns
+ *    in L, and no multiplication. */
+typedef enum ltxattn_rotary_scaling {
+  LTXATTN_ROTARY_NONE = 0,
+  LTXATTN_ROTARY_LINEAR = 1,
+  LTXATTN_ROTARY_NTK = 2,
+  LTXATTN_ROTARY_YARN = 3,
+  LTXATTN_ROTARY_BANDS = 4
+} ltxattn_rotary_scaling;
+
+/* Arguments of ltxattn_rotary_frequencies.  fast > slow > 0 and trained_length
+ * > 0 are needed by YARN and BANDS alone. */
+typedef struct ltxattn_rotary_frequency_args {
+  int32_t rotary_dim; /* even, >= 2 */
+  int32_t scaling;    /* ltxattn_rotary_scaling */
+  double theta;       /* > 0 and finite; > 1 for YARN */
+  double factor;      /* s > 0 (ignored by NONE) */
+  double trained_length;
+  double fast, slow;
+} ltxattn_rotary_frequency_args;
+
+/* Host arithmetic in double, no device work: writes rotary_dim / 2 angles per
+ * position step into `frequencies` (host memory, to be copied to the device
+ * once) and the factor on what is turned into *magnitude. */
+LTXATTN_API int ltxattn_rotary_frequencies(const ltxattn_rotary_frequency_args* args, double* frequencies,
+                                           float* magnitude);
+
+/* Arguments of ltxattn_rotary_embed: out = magnitude * R(position * frequency) x
+ * on the leading rotary_dim elements of every head of q and, with kv_heads > 0,
+ * of k (which may have fewer heads, as grouped-query attention has).
+ *  - q, q_out: [B, heads, T, D] views; k, k_out: [B, kv_heads, T, D].  An output
+ *    may be its input's own view (in place); it must not overlap an input in any
+ *    other way.  Inputs may repeat rows with zero strides, outputs may not.
+ *    Rows need no alignment; 16-byte aligned rows take the wide accesses.
+ *  - frequencies: device array of rotary_dim / 2 doubles.
+ *  - positions: device array, [B, T] with element strides (a zero stride_b
+ *    shares one row), int64 or int32 (position_bits 64 or 32), any sign; NULL:
+ *    token t stands at t.  `offset` is added to each position.
+ *  - inverse: turn the other way; with the same magnitude this is the gradient
+ *    (the transpose) of the call without it.
+ * Angles are formed and reduced to an eighth of a turn in fp64; cos and sin of
+ * the rest and the products are fp32, and each element is rounded once. */
+typedef struct ltxattn_rotary_embed_args {
+  int32_t dtype;
+  int32_t batch, tokens, heads, kv_heads, head_dim;
+  int32_t rotary_dim, layout, inverse;
+  float magnitude;
+  ltxattn_tensor q, q_out, k, k_out;
+  const double* frequencies;
+  const void* positions;
+  int32_t position_bits;
+  int64_t position_stride_b, position_stride_t;
+  int64_t offset;
+} ltxattn_rotary_embed_args;
+
+/* Rotates the queries and keys of an attention whose positions are token
+ * indices (grouped KV heads take no rotary inside ltxattn_fwd and are rotated
+ * by this call before it, the order of `GemmaTextEncoder.swift:173,193`), and
+ * their gradients after ltxattn_bwd.  One launch.  A batch, token or head count
+ * of zero is a call without work. */
+LTXATTN_API int ltxattn_rotary_embed(const ltxattn_rotary_embed_args* args, void* stream);
+
+/* ---- gated feed-forward block ----------------------------------------------- */
+
+typedef enum ltxattn_activation {
+  LTXATTN_SILU = 0,      /* g / (1 + e^-g) */
+  LTXATTN_GELU_TANH = 1, /* g/2 (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) */
+  LTXATTN_GELU = 2       /* g/2 (1 + erf(g / sqrt 2)) */
+} ltxattn_activation;
+
+/* Arguments of ltxattn_gated_ffn: out = (act(x w_gate^T) * (x w_up^T)) w_down^T.
+ *  - x [m, hidden], w_gate and w_up [inner, hidden], w_down [out_dim, inner],
+ *    out [m, out_dim]: bf16 rows of the given strides (elements), 16-byte
+ *    aligned; hidden, inner and out_dim multiples of 8; any m >= 0.
+ *  - gate, up: both NULL, or [m, inner] outputs that keep x w_gate^T and
+ *    x w_up^T (rounded to bf16) for the gradient.
+ *  - workspace: ltxattn_gated_ffn_workspace() bytes, 256-byte aligned; it holds
+ *    the product act(..) * (..) in bf16 between the two kernels. */
+typedef struct ltxattn_gated_ffn_args {
+  int32_t dtype; /* LTXATTN_BF16 */
+  int32_t activation;
+  int32_t m, hidden, inner, out_dim;
+  const void* x;
+  int64_t x_stride;
+  const void* w_gate;
+  int64_t w_gate_stride;
+  const void* w_up;
+  int64_t w_up_stride;
+  const void* w_down;
+  int64_t w_down_stride;
+  void* out;
+  int64_t out_stride;
+  void* gate;
+  int64_t gate_stride;
+  void* up;
+  int64_t up_stride;
+  void* workspace;
+  size_t workspace_bytes;
+} ltxattn_gated_ffn_args;
+
+/* The feed-forward half of a transformer block beside the attention half that
+ * ltxattn_linear and ltxattn_fwd make.  Both first projections, the activation
+ * and the product are one kernel (fp32 accumulators, one rounding of the
+ * product), the third projection a second one. */
+LTXATTN_API int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* args, void* stream);
+
+/* Device scratch bytes ltxattn_gated_ffn needs for these arguments. */
+LTXATTN_API size_t ltxattn_gated_ffn_workspace(const ltxattn_gated_ffn_args* args);
+
+/* Arguments of ltxattn_gated_ffn_bwd: from dout [m, out_dim] and the forward's
+ * gate and up, with h = act(gate) * up and dh = dout w_down,
+ *     dgate = dh * up * act'(gate),  dup = dh * act(gate),
+ *     dx = dgate w_gate + dup w_up,
+ *     dw_gate = dgate^T x,  dw_up = dup^T x,  dw_down = dout^T h.
+ * Each of dx [m, hidden], dw_gate, dw_up [inner, hidden] and dw_down
+ * [out_dim, inner] may be NULL, and is then not computed (frozen weights).
+ * x is read for dw_gate and dw_up alone, w_gate and w_up for dx alone: they may
+ * be NULL where those are.  Layout rules as for ltxattn_gated_ffn; with m = 0
+ * the weight gradients are set to zero.  Outputs must not overlap inputs or one
+ * another. */
+typedef struct ltxattn_gated_ffn_bwd_args {
+  int32_t dtype; /* LTXATTN_BF16 */
+  int32_t activation;
+  int32_t m, hidden, inner, out_dim;
+  const void* x;
+  int64_t x_stride;
+  const void* w_gate;
+  int64_t w_gate_stride;
+  const void* w_up;
+  int64_t w_up_stride;
+  const void* w_down;
+  int64_t w_down_stride;
+  const void* gate;
+  int64_t gate_stride;
+  const void* up;
+  int64_t up_stride;
+  const void* dout;
+  int64_t dout_stride;
+  void* dx;
+  int64_t dx_stride;
+  void* dw_gate;
+  int64_t dw_gate_stride;
+  void* dw_up;
+  int64_t dw_up_stride;
+  void* dw_down;
+  int64_t dw_down_stride;
+  void* workspace;
+  size_t workspace_bytes;
+} ltxattn_gated_ffn_bwd_args;
+
+LTXATTN_API int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* args, void* stream);
+
+/* Device scratch bytes ltxattn_gated_ffn_bwd needs for these arguments. */
+LTXATTN_API size_t ltxattn_gated_ffn_bwd_workspace(const ltxattn_gated_ffn_bwd_args* args);
+
 /* ---- query / key preparation ---------------------------------------------- */
 
 /* Arguments of ltxattn_qk_prep: out = split-RoPE(split(rmsNorm(x, weight))).

@@ -1,0 +1,666 @@
+// ffn_sm100.cu -- ltxattn_gated_ffn and ltxattn_gated_ffn_bwd: the gated
+// feed-forward block and its gradient on tcgen05 (sm_100a).
+//
+//   forward:   h = act(x Wg^T) * (x Wu^T)           one GEMM over [Wg; Wu], the product in its epilogue
+//              y = h Wd^T
+//   backward:  dh = dy Wd, and from it in the epilogue, with the kept gate g and up u,
+//              dg = dh u act'(g),  du = dh act(g),  h = act(g) u
+//              dx = dg Wg + du Wu                   one GEMM whose K runs through both pairs
+//              dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
+//
+// One persistent kernel, gemm_kernel<A major, B major, epilogue>, makes them
+// all: a CTA per SM walks over 128 x 256 output tiles (fp32 in TMEM).  Warp 0
+// lane 0 loads 64-wide K slices of both operands with TMA into a ring of
+// shared-memory stages (128-byte swizzle), warp 1 lane 0 issues the MMAs, and
+// warps 4-11 turn the finished accumulator into the output while the next
+// tile's MMAs fill the other half of TMEM.
+//
+// Operands that lie along the wrong axis (the weights of dh and dx, both
+// operands of the weight gradients) are read as they lie: their tiles are
+// staged as 64-element chunks of the row/column axis and the MMA takes them
+// MN-major, so nothing is transposed through memory.
+//
+// Sizes that fill no tile need no case of their own: TMA reads zeros outside a
+// tensor (also for the rest of K), and the epilogue stores only what exists.
+//
+// Roundings: accumulators are fp32.  h, dg and du are rounded to bf16 once,
+// because the tensor cores take them as bf16 operands of the next product; the
+// outputs are rounded once.
+//
+// Bound: the tensor cores (at 3120 x 4096 x 16384 the forward does 2770
+// operations per byte it must move).
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <mutex>
+
+#include "../../include/ltxattn.h"
+#include "ltxattn_internal.h"
+#include "sm100.cuh"
+
+namespace ltx {
+
+int set_error_message(int status, const char* msg);
+
+namespace {
+
+constexpr int kGM = 128;       // rows of a tile (UMMA M)
+constexpr int kGN = 256;       // accumulator columns of a tile (UMMA N)
+constexpr int kGK = 64;        // K per stage: one 128-byte swizzle row of bf16
+constexpr int kGStages = 4;
+constexpr int kGThreads = 384;  // 4 control warps, 8 epilogue warps
+constexpr uint32_t kGA = kGM * kGK * 2;
+constexpr uint32_t kGB = kGN * kGK * 2;
+constexpr uint32_t kGStage = kGA + kGB;
+constexpr uint32_t kChunk = 64 * kGK * 2;  // MN-major: 64 columns x 64 rows of K
+// full[kGStages], empty[kGStages], acc_full[2], acc_empty[2]
+constexpr uint32_t kGOffBar = kGStages * kGStage;
+constexpr uint32_t kGOffCtl = kGOffBar + (2 * kGStages + 4) * 8;  // TMEM slot, abort flag
+constexpr uint32_t kGSmem = kGOffCtl + 16 + 1024;                 // + alignment slack
+constexpr int kGEpilogueThreads = 256;
+
+enum Epilogue { kProduct, kStore, kSlopes };
+
+// One output of a launch (a launch of the weight gradients has up to three).
+struct Gemm {
+  CUtensorMap a[2], b[2];  // K slices beyond kb_first come from the second pair
+  int M, N;                // rows and accumulator columns that exist (kProduct: columns of h)
+  int kb, kb_first;        // 64-wide K slices in all, and those of the first pair
+  int tiles_m, tiles_n;
+  __nv_bfloat16* out;
+  int64_t out_stride;
+};
+
+struct GemmParams {
+  Gemm g[3];
+  int first_tile[4];  // tiles of g[i]: [first_tile[i], first_tile[i + 1])
+  int count;
+  int activation;
+  // kProduct: gate and up to be kept (or null).  kSlopes: the kept ones, and dgate and dup
+  __nv_bfloat16 *gate, *up, *dgate, *dup;
+  int64_t gate_stride, up_stride, dgate_stride, dup_stride;
+  int* err;
+};
+
+// ---------------------------------------------------------------------------
+// activations (fp32)
+
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
+
+// act(g), and with kSlope its derivative too.
+template <bool kSlope>
+__device__ __forceinline__ float activate(int kind, float g, float& slope) {
+  if (kind == LTXATTN_SILU) {
+    const float s = sigmoid(g);
+    if (kSlope) slope = s * fmaf(g, 1.0f - s, 1.0f);
+    return g * s;
+  }
+  if (kind == LTXATTN_GELU_TANH) {
+    // (1 + tanh z) / 2 = sigmoid(2 z)
+    constexpr float c2 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+    const float g2 = g * g;
+    const float s = sigmoid(c2 * g * fmaf(0.044715f, g2, 1.0f));
+    if (kSlope) {
+      const float t = g * s * (1.0f - s);  // 0 far out, where g2 may be infinite
+      slope = t == 0.0f ? s : fmaf(t, c2 * fmaf(0.134145f, g2, 1.0f), s);
+    }
+    return g * s;
+  }
+  const float s = 0.5f * erfcf(-0.70710678118654752f * g);
+  if (kSlope) slope = fmaf(g, 0.3989422804014327f * __expf(-0.5f * g * g), s);
+  return g * s;
+}
+
+__device__ __forceinline__ float lo_f(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float hi_f(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// 8 consecutive bf16 of a row (16-byte aligned).
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                                            pack_bf16x2(v[6], v[7]));
+}
+
+// ---------------------------------------------------------------------------
+
+// Tiles are numbered down the rows first, in bands of kBand row blocks: the CTAs
+// that run together then share a few column blocks of B and the band's rows of A.
+constexpr int kBand = 16;
+
+__device__ __forceinline__ void locate(const GemmParams& p, int tile, int& which, int& m0, int& tn) {
+  which = 0;
+  while (which + 1 < p.count && tile >= p.first_tile[which + 1]) ++which;
+  const Gemm& g = p.g[which];
+  const int i = tile - p.first_tile[which];
+  const int band = i / (kBand * g.tiles_n);
+  const int rows = min(kBand, g.tiles_m - band * kBand);
+  const int j = i - band * kBand * g.tiles_n;
+  m0 = (band * kBand + j % rows) * kGM;
+  tn = j / rows;
+}
+
+template <bool kAMN, bool kBMN, int kEpilogue>
+__global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = align1024(smem_raw);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + kGOffBar);
+  uint64_t* empty = full + kGStages;
+  uint64_t* acc_full = empty + kGStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + kGOffCtl);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + kGOffCtl + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = p.first_tile[p.count];
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2 * kGStages; ++i) mbar_init(full + i, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + i, 1);
+      mbar_init(acc_empty + i, kGEpilogueThreads / 32);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    int it = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      int which, m0, tn;
+      locate(p, tile, which, m0, tn);
+      const Gemm& g = p.g[which];
+      for (int kb = 0; kb < g.kb; ++kb, ++it) {
+        const int st = it % kGStages, u = it / kGStages;
+        if (it >= kGStages && !mbar_wait(empty + st, (u - 1) & 1, abort_flag, p.err, 61)) {
+          ok = false;
+          break;
+        }
+        uint8_t* sa = sm + st * kGStage;
+        uint8_t* sb = sa + kGA;
+        const int part = kb >= g.kb_first;
+        const int k0 = (part ? kb - g.kb_first : kb) * kGK;
+        mbar_arrive_expect_tx(full + st, kGStage);
+        if (kAMN) {
+#pragma unroll
+          for (int c = 0; c < kGM / 64; ++c) tma_load_2d(&g.a[part], full + st, sa + c * kChunk, m0 + c * 64, k0);
+        } else {
+          tma_load_2d(&g.a[part], full + st, sa, k0, m0);
+        }
+        if (kEpilogue == kProduct) {
+          // rows 0-127 of the B tile are the gate's weights, rows 128-255 the up projection's
+          tma_load_2d(&g.b[0], full + st, sb, k0, tn * (kGN / 2));
+          tma_load_2d(&g.b[1], full + st, sb + kGB / 2, k0, tn * (kGN / 2));
+        } else if (kBMN) {
+#pragma unroll
+          for (int c = 0; c < kGN / 64; ++c)
+            tma_load_2d(&g.b[part], full + st, sb + c * kChunk, tn * kGN + c * 64, k0);
+        } else {
+          tma_load_2d(&g.b[part], full + st, sb, k0, tn * kGN);
+        }
+      }
+    }
+    // never leave the CTA with a bulk copy still writing its shared memory
+    for (int i = it < kGStages ? 0 : it - kGStages; i < it; ++i) drain_wait(full + i % kGStages, (i / kGStages) & 1);
+  } else if (warp == 1 && lane == 0) {
+    constexpr uint32_t idesc = idesc_bf16_f32(kGM, kGN, kAMN, kBMN);
+    const SDesc a0 = sdesc_split(smem_u32(sm), kAMN ? kChunk : 16, 1024);
+    const SDesc b0 = sdesc_split(smem_u32(sm) + kGA, kBMN ? kChunk : 16, 1024);
+    // 16 of K further along: 32 bytes of each row K-major, 16 rows of 128 bytes MN-major
+    constexpr uint32_t a_step = kAMN ? 128 : 2, b_step = kBMN ? 128 : 2;
+    int it = 0, n = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
+      int which, m0, tn;
+      locate(p, tile, which, m0, tn);
+      const int kb_n = p.g[which].kb;
+      const int buf = n & 1;
+      if (n >= 2 && !mbar_wait(acc_empty + buf, ((n >> 1) - 1) & 1, abort_flag, p.err, 62)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + buf * kGN;
+      for (int kb = 0; kb < kb_n; ++kb, ++it) {
+        const int st = it % kGStages, u = it / kGStages;
+        if (!mbar_wait(full + st, u & 1, abort_flag, p.err, 63)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t alo = a0.lo + st * (kGStage >> 4), blo = b0.lo + st * (kGStage >> 4);
+#pragma unroll
+        for (int kk = 0; kk < kGK / 16; ++kk)
+          umma_ss2(d, alo + kk * a_step, a0.hi, blo + kk * b_step, b0.hi, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(empty + st);  // the stage is free once these MMAs have read it
+      }
+      umma_commit(acc_full + buf);
+    }
+    // no MMA still running when the CTA tears down: the last commits cover all of them
+    for (int i = n < 2 ? 0 : n - 2; i < n; ++i) drain_wait(acc_full + (i & 1), (i >> 1) & 1);
+  } else if (warp >= 4) {
+    const int quadrant = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t lane_off = static_cast<uint32_t>(quadrant * 32) << 16;
+    int n = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+      int which, m0, tn;
+      locate(p, tile, which, m0, tn);
+      const Gemm& g = p.g[which];
+      const int buf = n & 1;
+      if (!warp_wait(acc_full + buf, (n >> 1) & 1, abort_flag, p.err, 64)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + buf * kGN + lane_off;
+      const int64_t row = m0 + quadrant * 32 + lane;
+      const bool exists = row < g.M;
+      if (kEpilogue == kProduct) {
+        // 64 columns of h per warp: accumulator columns c (gate) and 128 + c (up)
+#pragma unroll 1
+        for (int c = half * 64; c < half * 64 + 64; c += 16) {
+          const int col = tn * (kGN / 2) + c;
+          if (col >= g.N) break;  // warp-uniform
+          __syncwarp();
+          uint32_t rg[16], ru[16];
+          tmem_ld16(d + c, rg);
+          tmem_ld16(d + kGN / 2 + c, ru);
+          tmem_wait_ld();
+          if (!exists) continue;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            if (col + 8 * q >= g.N) break;
+            float v[8], gv[8], uv[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              gv[e] = __uint_as_float(rg[8 * q + e]);
+              uv[e] = __uint_as_float(ru[8 * q + e]);
+              float unused;
+              v[e] = activate<false>(p.activation, gv[e], unused) * uv[e];
+            }
+            store8(g.out + row * g.out_stride + col + 8 * q, v);
+            if (p.gate != nullptr) {
+              store8(p.gate + row * p.gate_stride + col + 8 * q, gv);
+              store8(p.up + row * p.up_stride + col + 8 * q, uv);
+            }
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = half * 128; c < half * 128 + 128; c += 32) {
+          const int col = tn * kGN + c;
+          if (col >= g.N) break;  // warp-uniform
+          __syncwarp();
+          uint32_t r[32];
+          tmem_ld32(d + c, r);
+          tmem_wait_ld();
+          if (!exists) continue;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (col + 8 * q >= g.N) break;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[8 * q + e]);
+            if (kEpilogue == kSlopes) {
+              const uint4 g4 = *reinterpret_cast<const uint4*>(p.gate + row * p.gate_stride + col + 8 * q);
+              const uint4 u4 = *reinterpret_cast<const uint4*>(p.up + row * p.up_stride + col + 8 * q);
+              const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
+              float dgv[8], duv[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float gv = (e & 1) ? hi_f(gw[e / 2]) : lo_f(gw[e / 2]);
+                const float uv = (e & 1) ? hi_f(uw[e / 2]) : lo_f(uw[e / 2]);
+                float slope;
+                const float a = activate<true>(p.activation, gv, slope);
+                dgv[e] = v[e] * uv * slope;
+                duv[e] = v[e] * a;
+                v[e] = a * uv;
+              }
+              store8(p.dgate + row * p.dgate_stride + col + 8 * q, dgv);
+              store8(p.dup + row * p.dup_stride + col + 8 * q, duv);
+              if (g.out == nullptr) continue;  // h is wanted for dw_down alone
+            }
+            store8(g.out + row * g.out_stride + col + 8 * q, v);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty + buf);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encoder() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(f);
+    else
+      (void)cudaGetLastError();
+  });
+  return fn;
+}
+
+int fail_ffn(int status, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return set_error_message(status, buf);
+}
+
+// bf16 [rows, cols], `stride` elements between rows; boxes of 64 columns (one swizzle row) and box_rows rows.
+int map_2d(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t stride, int box_rows,
+           const char* name) {
+  EncodeTiledFn enc = encoder();
+  if (!enc) return fail_ffn(LTXATTN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail_ffn(LTXATTN_ERR_ALIGN, "%s: cuTensorMapEncodeTiled rejected the view (CUresult %d)", name, (int)r);
+  return LTXATTN_OK;
+}
+
+// A bf16 matrix argument.
+struct Mat {
+  const char* name;
+  const void* data;
+  int64_t stride;
+  int64_t rows, cols;
+};
+
+int check_mat(const char* call, const Mat& m) {
+  if (m.data == nullptr) return fail_ffn(LTXATTN_ERR_ARG, "%s: %s is required", call, m.name);
+  if (m.stride < m.cols)
+    return fail_ffn(LTXATTN_ERR_SHAPE, "%s: %s's row stride (%lld) is shorter than its row (%lld)", call, m.name,
+                    (long long)m.stride, (long long)m.cols);
+  if ((reinterpret_cast<uintptr_t>(m.data) & 15u) || m.stride % 8)
+    return fail_ffn(LTXATTN_ERR_ALIGN, "%s: %s needs 16-byte aligned rows", call, m.name);
+  if (m.stride > (int64_t(1) << 38))
+    return fail_ffn(LTXATTN_ERR_UNSUPPORTED, "%s: %s's row stride is too large", call, m.name);
+  return LTXATTN_OK;
+}
+
+int check_sizes(const char* call, int dtype, int activation, int m, int hidden, int inner, int out_dim) {
+  if (dtype != LTXATTN_BF16) return fail_ffn(LTXATTN_ERR_DTYPE, "%s: bf16 only", call);
+  if (activation < LTXATTN_SILU || activation > LTXATTN_GELU)
+    return fail_ffn(LTXATTN_ERR_ARG, "%s: unknown activation %d", call, activation);
+  if (m < 0 || hidden < 1 || inner < 1 || out_dim < 1)
+    return fail_ffn(LTXATTN_ERR_SHAPE, "%s: m must be >= 0, hidden, inner and out_dim >= 1", call);
+  if (hidden % 8 || inner % 8 || out_dim % 8)
+    return fail_ffn(LTXATTN_ERR_UNSUPPORTED, "%s: hidden (%d), inner (%d) and out_dim (%d) must be multiples of 8", call,
+                    hidden, inner, out_dim);
+  return LTXATTN_OK;
+}
+
+constexpr int kMaxDev = 64;
+std::mutex g_mu;
+bool g_attr_set[kMaxDev][8] = {};
+int g_sms[kMaxDev] = {};
+
+// The SM count, with the kernel's shared memory opted into once per device.
+template <typename K>
+cudaError_t prepare_kernel(K kernel, int slot, int* sms) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDev) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(g_mu);
+  if (!g_attr_set[dev][slot]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGSmem);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    g_attr_set[dev][slot] = true;
+  }
+  *sms = g_sms[dev];
+  return cudaSuccess;
+}
+
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <bool kAMN, bool kBMN, int kEpilogue>
+int launch_gemm(GemmParams& p, int slot, const char* call, cudaStream_t st) {
+  const int width = kEpilogue == kProduct ? kGN / 2 : kGN;
+  int64_t tiles = 0;
+  for (int i = 0; i < p.count; ++i) {
+    Gemm& g = p.g[i];
+    g.tiles_m = (int)div_up(g.M, kGM);
+    g.tiles_n = (int)div_up(g.N, width);
+    p.first_tile[i] = (int)tiles;
+    tiles += (int64_t)g.tiles_m * g.tiles_n;
+    if (tiles > 0x3fffffff) return fail_ffn(LTXATTN_ERR_UNSUPPORTED, "%s: too many output tiles", call);
+  }
+  p.first_tile[p.count] = (int)tiles;
+  p.err = device_error_word();
+  if (!p.err) return fail_ffn(LTXATTN_ERR_CUDA, "no device error word");
+  int sms = 0;
+  cudaError_t e = prepare_kernel(gemm_kernel<kAMN, kBMN, kEpilogue>, slot, &sms);
+  if (e == cudaSuccess) {
+    gemm_kernel<kAMN, kBMN, kEpilogue>
+        <<<(unsigned)std::min<int64_t>(tiles, sms), kGThreads, kGSmem, st>>>(p);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail_ffn(LTXATTN_ERR_CUDA, "%s: %s", call, cudaGetErrorString(e));
+  }
+  return LTXATTN_OK;
+}
+
+size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// h, dgate and dup between the kernels: [m, inner] bf16 with contiguous rows.
+size_t plane_bytes(int m, int inner) { return round256((size_t)m * inner * 2); }
+
+int check_workspace(const char* call, const void* ws, size_t have, size_t need) {
+  if (ws == nullptr || have < need)
+    return fail_ffn(LTXATTN_ERR_WORKSPACE, "%s: the workspace has %zu bytes, %zu are needed", call, ws ? have : 0, need);
+  if (reinterpret_cast<uintptr_t>(ws) & 255u)
+    return fail_ffn(LTXATTN_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", call);
+  return LTXATTN_OK;
+}
+
+}  // namespace
+}  // namespace ltx
+
+using namespace ltx;
+
+extern "C" {
+
+size_t ltxattn_gated_ffn_workspace(const ltxattn_gated_ffn_args* a) {
+  if (a == nullptr || a->m < 1 || a->inner < 1) return 0;
+  return plane_bytes(a->m, a->inner);
+}
+
+int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
+  const char* call = "ltxattn_gated_ffn";
+  if (a == nullptr) return fail_ffn(LTXATTN_ERR_ARG, "args is NULL");
+  if (int rc = check_sizes(call, a->dtype, a->activation, a->m, a->hidden, a->inner, a->out_dim)) return rc;
+  if ((a->gate == nullptr) != (a->up == nullptr) && a->m > 0)
+    return fail_ffn(LTXATTN_ERR_ARG, "%s: gate and up are kept together or not at all", call);
+  if (a->m == 0) return LTXATTN_OK;
+  const Mat mats[7] = {{"x", a->x, a->x_stride, a->m, a->hidden},
+                       {"w_gate", a->w_gate, a->w_gate_stride, a->inner, a->hidden},
+                       {"w_up", a->w_up, a->w_up_stride, a->inner, a->hidden},
+                       {"w_down", a->w_down, a->w_down_stride, a->out_dim, a->inner},
+                       {"out", a->out, a->out_stride, a->m, a->out_dim},
+                       {"gate", a->gate, a->gate_stride, a->m, a->inner},
+                       {"up", a->up, a->up_stride, a->m, a->inner}};
+  for (int i = 0; i < (a->gate ? 7 : 5); ++i)
+    if (int rc = check_mat(call, mats[i])) return rc;
+  if (int rc = check_workspace(call, a->workspace, a->workspace_bytes, ltxattn_gated_ffn_workspace(a))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  __nv_bfloat16* h = static_cast<__nv_bfloat16*>(a->workspace);
+
+  GemmParams p{};
+  p.count = 1;
+  p.activation = a->activation;
+  Gemm& g = p.g[0];
+  if (int rc = map_2d(&g.a[0], a->x, a->m, a->hidden, a->x_stride, kGM, "x")) return rc;
+  if (int rc = map_2d(&g.b[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, kGN / 2, "w_gate")) return rc;
+  if (int rc = map_2d(&g.b[1], a->w_up, a->inner, a->hidden, a->w_up_stride, kGN / 2, "w_up")) return rc;
+  g.M = a->m;
+  g.N = a->inner;
+  g.kb = g.kb_first = (int)div_up(a->hidden, kGK);
+  g.out = h;
+  g.out_stride = a->inner;
+  p.gate = static_cast<__nv_bfloat16*>(a->gate);
+  p.up = static_cast<__nv_bfloat16*>(a->up);
+  p.gate_stride = a->gate_stride;
+  p.up_stride = a->up_stride;
+  if (int rc = launch_gemm<false, false, kProduct>(p, 0, call, st)) return rc;
+
+  GemmParams d{};
+  d.count = 1;
+  Gemm& o = d.g[0];
+  if (int rc = map_2d(&o.a[0], h, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
+  if (int rc = map_2d(&o.b[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, kGN, "w_down")) return rc;
+  o.M = a->m;
+  o.N = a->out_dim;
+  o.kb = o.kb_first = (int)div_up(a->inner, kGK);
+  o.out = static_cast<__nv_bfloat16*>(a->out);
+  o.out_stride = a->out_stride;
+  return launch_gemm<false, false, kStore>(d, 1, call, st);
+}
+
+size_t ltxattn_gated_ffn_bwd_workspace(const ltxattn_gated_ffn_bwd_args* a) {
+  if (a == nullptr || a->m < 1 || a->inner < 1) return 0;
+  return 3 * plane_bytes(a->m, a->inner);
+}
+
+int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
+  const char* call = "ltxattn_gated_ffn_bwd";
+  if (a == nullptr) return fail_ffn(LTXATTN_ERR_ARG, "args is NULL");
+  if (int rc = check_sizes(call, a->dtype, a->activation, a->m, a->hidden, a->inner, a->out_dim)) return rc;
+  const bool dw_in = a->dw_gate != nullptr || a->dw_up != nullptr;
+  const Mat outs[4] = {{"dx", a->dx, a->dx_stride, a->m, a->hidden},
+                       {"dw_gate", a->dw_gate, a->dw_gate_stride, a->inner, a->hidden},
+                       {"dw_up", a->dw_up, a->dw_up_stride, a->inner, a->hidden},
+                       {"dw_down", a->dw_down, a->dw_down_stride, a->out_dim, a->inner}};
+  bool any = false;
+  for (int i = 0; i < 4; ++i) {
+    if (outs[i].data == nullptr || (i == 0 && a->m == 0)) continue;
+    any = true;
+    if (int rc = check_mat(call, outs[i])) return rc;
+  }
+  if (!any) return LTXATTN_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->m == 0) {  // no tokens: the weights' gradients are sums of nothing
+    for (int i = 1; i < 4; ++i) {
+      if (outs[i].data == nullptr) continue;
+      const cudaError_t e = cudaMemset2DAsync(const_cast<void*>(outs[i].data), (size_t)outs[i].stride * 2, 0,
+                                              (size_t)outs[i].cols * 2, (size_t)outs[i].rows, st);
+      if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return fail_ffn(LTXATTN_ERR_CUDA, "%s: %s", call, cudaGetErrorString(e));
+      }
+    }
+    return LTXATTN_OK;
+  }
+  const Mat ins[7] = {{"gate", a->gate, a->gate_stride, a->m, a->inner},
+                      {"up", a->up, a->up_stride, a->m, a->inner},
+                      {"dout", a->dout, a->dout_stride, a->m, a->out_dim},
+                      {"w_down", a->w_down, a->w_down_stride, a->out_dim, a->inner},
+                      {"w_gate", a->w_gate, a->w_gate_stride, a->inner, a->hidden},
+                      {"w_up", a->w_up, a->w_up_stride, a->inner, a->hidden},
+                      {"x", a->x, a->x_stride, a->m, a->hidden}};
+  for (int i = 0; i < 7; ++i) {
+    if ((i == 4 || i == 5) && a->dx == nullptr) continue;
+    if (i == 6 && !dw_in) continue;
+    if (int rc = check_mat(call, ins[i])) return rc;
+  }
+  if (int rc = check_workspace(call, a->workspace, a->workspace_bytes, ltxattn_gated_ffn_bwd_workspace(a))) return rc;
+  const size_t plane = plane_bytes(a->m, a->inner);
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  __nv_bfloat16* dgate = reinterpret_cast<__nv_bfloat16*>(ws);
+  __nv_bfloat16* dup = reinterpret_cast<__nv_bfloat16*>(ws + plane);
+  __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(ws + 2 * plane);
+
+  {  // dh = dout w_down, and what follows from it element by element
+    GemmParams p{};
+    p.count = 1;
+    p.activation = a->activation;
+    Gemm& g = p.g[0];
+    if (int rc = map_2d(&g.a[0], a->dout, a->m, a->out_dim, a->dout_stride, kGM, "dout")) return rc;
+    if (int rc = map_2d(&g.b[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, kGK, "w_down")) return rc;
+    g.M = a->m;
+    g.N = a->inner;
+    g.kb = g.kb_first = (int)div_up(a->out_dim, kGK);
+    g.out = a->dw_down != nullptr ? h : nullptr;
+    g.out_stride = a->inner;
+    p.gate = static_cast<__nv_bfloat16*>(const_cast<void*>(a->gate));
+    p.up = static_cast<__nv_bfloat16*>(const_cast<void*>(a->up));
+    p.gate_stride = a->gate_stride;
+    p.up_stride = a->up_stride;
+    p.dgate = dgate;
+    p.dup = dup;
+    p.dgate_stride = p.dup_stride = a->inner;
+    if (int rc = launch_gemm<false, true, kSlopes>(p, 2, call, st)) return rc;
+  }
+  if (a->dx != nullptr) {
+    GemmParams p{};
+    p.count = 1;
+    Gemm& g = p.g[0];
+    if (int rc = map_2d(&g.a[0], dgate, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
+    if (int rc = map_2d(&g.a[1], dup, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
+    if (int rc = map_2d(&g.b[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, kGK, "w_gate")) return rc;
+    if (int rc = map_2d(&g.b[1], a->w_up, a->inner, a->hidden, a->w_up_stride, kGK, "w_up")) return rc;
+    g.M = a->m;
+    g.N = a->hidden;
+    g.kb_first = (int)div_up(a->inner, kGK);
+    g.kb = 2 * g.kb_first;
+    g.out = static_cast<__nv_bfloat16*>(a->dx);
+    g.out_stride = a->dx_stride;
+    if (int rc = launch_gemm<false, true, kStore>(p, 3, call, st)) return rc;
+  }
+  GemmParams p{};
+  auto weight = [&](const void* at, int64_t at_stride, int rows, const void* b, int64_t b_stride, int cols, void* out,
+                    int64_t out_stride, const char* an, const char* bn) {
+    if (out == nullptr) return (int)LTXATTN_OK;
+    Gemm& g = p.g[p.count++];
+    if (int rc = map_2d(&g.a[0], at, a->m, rows, at_stride, kGK, an)) return rc;
+    if (int rc = map_2d(&g.b[0], b, a->m, cols, b_stride, kGK, bn)) return rc;
+    g.M = rows;
+    g.N = cols;
+    g.kb = g.kb_first = (int)div_up(a->m, kGK);
+    g.out = static_cast<__nv_bfloat16*>(out);
+    g.out_stride = out_stride;
+    return (int)LTXATTN_OK;
+  };
+  if (int rc = weight(dgate, a->inner, a->inner, a->x, a->x_stride, a->hidden, a->dw_gate, a->dw_gate_stride,
+                      "workspace", "x"))
+    return rc;
+  if (int rc = weight(dup, a->inner, a->inner, a->x, a->x_stride, a->hidden, a->dw_up, a->dw_up_stride, "workspace", "x"))
+    return rc;
+  if (int rc = weight(a->dout, a->dout_stride, a->out_dim, h, a->inner, a->inner, a->dw_down, a->dw_down_stride, "dout",
+                      "workspace"))
+    return rc;
+  if (p.count == 0) return LTXATTN_OK;
+  return launch_gemm<true, true, kStore>(p, 4, call, st);
+}
+
+}  // extern "C"

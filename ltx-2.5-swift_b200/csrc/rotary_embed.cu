@@ -1,0 +1,343 @@
+// rotary_embed.cu -- ltxattn_rotary_embed and ltxattn_rotary_frequencies:
+// rotary positions from token indices, for the queries and (grouped) keys of
+// one attention in one launch, and their gradients.
+//
+//   (a, b) -> magnitude * (a cos w - b sin w,  b cos w + a sin w),  w = position * frequency
+//
+// for every pair of the leading rotary_dim elements of a head; the inverse call
+// takes -w.  All heads of a token turn by the same angles, so a thread owns one
+// slot of a token (kP pairs, or kP elements behind the rotary part) and walks
+// over heads with cos and sin in registers.
+//
+// Angle: w reaches 1e6 radians at far positions, where fp32 keeps no fraction
+// of a turn.  The number of turns is formed in fp64 and reduced there to
+// [-1/8, 1/8] plus a quarter count; only that remainder (rounded to fp32:
+// 2^-28 turns at most) goes through sincospif, and the quarters are sign and
+// swap selects.  Products are fp32; each element is rounded once.
+//
+// Bound: memory.  q and k are read once and written once, and nothing else has
+// their size.
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+#include "../../include/ltxattn.h"
+#include "ltxattn_internal.h"
+#include "sm100.cuh"
+
+namespace ltx {
+
+int set_error_message(int status, const char* msg);
+
+namespace {
+
+constexpr int kRThreads = 256;
+constexpr int kRUnroll = 4;  // heads whose loads are in flight together
+
+struct RView {
+  const void* x;
+  void* y;
+  int64_t x_sb, x_sh, x_st;
+  int64_t y_sb, y_sh, y_st;
+};
+
+struct RotaryEmbedParams {
+  RView v[2];  // q, k
+  int heads, total_heads;  // q's, and q's and k's together
+  int T, pairs;
+  unsigned items;       // B * T * slots
+  int slots;            // slots of a token: turned ones, then copied ones
+  int turn_slots;       // pairs / kP
+  int heads_per_thread;
+  const double* freq;
+  const void* positions;  // or null: token t stands at t
+  int pos64;
+  int64_t pos_sb, pos_st, offset;
+  float magnitude;
+  int inverse;
+};
+
+template <typename T, int kN>
+struct alignas(sizeof(T) * kN <= 16 ? sizeof(T) * kN : 16) Vec {
+  T e[kN];
+};
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_f(float& d, float v) { d = v; }
+__device__ __forceinline__ void from_f(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
+
+// cos and sin of position * frequency (see the head of the file).
+__device__ __forceinline__ void turn(double position, double frequency, float& c, float& s) {
+  const double turns = position * frequency * 0.15915494309189533577;  // 1 / (2 pi)
+  const double part = turns - rint(turns);
+  const double quarter = rint(4.0 * part);
+  float cr, sr;
+  sincospif(2.0f * static_cast<float>(part - 0.25 * quarter), &sr, &cr);
+  const int q = static_cast<int>(quarter) & 3;
+  const float c1 = (q & 1) ? -sr : cr, s1 = (q & 1) ? cr : sr;
+  c = (q & 2) ? -c1 : c1;
+  s = (q & 2) ? -s1 : s1;
+}
+
+// kP pairs per turned slot.  Half layout: two runs of kP elements, `pairs`
+// apart; interleaved: one run of 2 kP.  Copied slots are runs of kP.
+template <typename T, int kP, bool kInterleaved>
+__global__ void __launch_bounds__(kRThreads) rotary_embed_kernel(const __grid_constant__ RotaryEmbedParams p) {
+  const unsigned i = blockIdx.x * kRThreads + threadIdx.x;
+  if (i >= p.items) return;
+  const unsigned slot = i % p.slots, bt = i / p.slots;
+  const int t = static_cast<int>(bt % p.T), b = static_cast<int>(bt / p.T);
+  const int h0 = blockIdx.y * p.heads_per_thread;
+  const int h1 = min(h0 + p.heads_per_thread, p.total_heads);
+  using Run = Vec<T, kP>;
+  const bool turned = slot < static_cast<unsigned>(p.turn_slots);
+
+  float c[kP], s[kP];
+  int at0, at1;  // the slot's two runs in a head (a copied slot has the first alone)
+  if (turned) {
+    int64_t place = t;
+    if (p.positions != nullptr) {
+      const int64_t o = b * p.pos_sb + t * p.pos_st;
+      place = p.pos64 ? static_cast<const int64_t*>(p.positions)[o] : static_cast<const int32_t*>(p.positions)[o];
+    }
+    const double position = static_cast<double>(place + p.offset);
+#pragma unroll
+    for (int e = 0; e < kP; ++e) {
+      turn(position, p.freq[slot * kP + e], c[e], s[e]);
+      c[e] *= p.magnitude;
+      s[e] *= p.inverse ? -p.magnitude : p.magnitude;
+    }
+    at0 = kInterleaved ? 2 * kP * slot : kP * slot;
+    at1 = kInterleaved ? at0 + kP : at0 + p.pairs;
+  } else {
+    at0 = 2 * p.pairs + kP * (slot - p.turn_slots);
+    at1 = at0;
+  }
+
+  for (int h = h0; h < h1; h += kRUnroll) {
+    Run r0[kRUnroll], r1[kRUnroll];
+#pragma unroll
+    for (int u = 0; u < kRUnroll; ++u) {
+      if (h + u >= h1) break;
+      const bool k = h + u >= p.heads;
+      const RView& v = p.v[k];
+      const T* x = static_cast<const T*>(v.x) + b * v.x_sb + (int64_t)(k ? h + u - p.heads : h + u) * v.x_sh +
+                   (int64_t)t * v.x_st;
+      r0[u] = *reinterpret_cast<const Run*>(x + at0);
+      if (turned) r1[u] = *reinterpret_cast<const Run*>(x + at1);
+    }
+#pragma unroll
+    for (int u = 0; u < kRUnroll; ++u) {
+      if (h + u >= h1) break;
+      const bool k = h + u >= p.heads;
+      const RView& v = p.v[k];
+      T* y = static_cast<T*>(v.y) + b * v.y_sb + (int64_t)(k ? h + u - p.heads : h + u) * v.y_sh + (int64_t)t * v.y_st;
+      if (turned) {
+#pragma unroll
+        for (int e = 0; e < kP; ++e) {
+          // interleaved: pair e is elements 2e and 2e + 1 of the two runs taken as one
+          T& ea = !kInterleaved ? r0[u].e[e] : 2 * e < kP ? r0[u].e[(2 * e) % kP] : r1[u].e[(2 * e) % kP];
+          T& eb = !kInterleaved ? r1[u].e[e] : 2 * e + 1 < kP ? r0[u].e[(2 * e + 1) % kP] : r1[u].e[(2 * e + 1) % kP];
+          const float fa = to_f(ea), fb = to_f(eb);
+          from_f(ea, fmaf(fa, c[e], -(fb * s[e])));
+          from_f(eb, fmaf(fb, c[e], fa * s[e]));
+        }
+        *reinterpret_cast<Run*>(y + at1) = r1[u];
+      }
+      *reinterpret_cast<Run*>(y + at0) = r0[u];
+    }
+  }
+}
+
+int fail_rotary(int status, const char* fmt, ...) {
+  char buf[256];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return set_error_message(status, buf);
+}
+
+template <typename T, int kP>
+void launch(const RotaryEmbedParams& p, bool interleaved, dim3 grid, cudaStream_t st) {
+  if (interleaved)
+    rotary_embed_kernel<T, kP, true><<<grid, kRThreads, 0, st>>>(p);
+  else
+    rotary_embed_kernel<T, kP, false><<<grid, kRThreads, 0, st>>>(p);
+}
+
+// Whether every row of the view starts on a multiple of `elements` elements.  The
+// stride of an extent of 1 is never used.
+bool rows_aligned(const ltxattn_tensor& v, int64_t B, int64_t H, int64_t T, int elements, int size) {
+  return reinterpret_cast<uintptr_t>(v.data) % (elements * size) == 0 && (B == 1 || v.stride_b % elements == 0) &&
+         (H == 1 || v.stride_h % elements == 0) && (T == 1 || v.stride_t % elements == 0);
+}
+
+// Checks one input and its output; 0 or the status that fail_rotary gave.
+int check_view(const char* name, const ltxattn_tensor& x, const ltxattn_tensor& y, int64_t B, int64_t H, int64_t T,
+               int size) {
+  if (x.data == nullptr || y.data == nullptr)
+    return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_embed: %s and its output are required", name);
+  if (reinterpret_cast<uintptr_t>(x.data) % size || reinterpret_cast<uintptr_t>(y.data) % size)
+    return fail_rotary(LTXATTN_ERR_ALIGN, "ltxattn_rotary_embed: %s is not aligned to its type", name);
+  if (x.stride_b < 0 || x.stride_h < 0 || x.stride_t < 0 || y.stride_b < 0 || y.stride_h < 0 || y.stride_t < 0)
+    return fail_rotary(LTXATTN_ERR_SHAPE, "ltxattn_rotary_embed: %s has a negative stride", name);
+  if ((B > 1 && y.stride_b == 0) || (H > 1 && y.stride_h == 0) || (T > 1 && y.stride_t == 0))
+    return fail_rotary(LTXATTN_ERR_SHAPE, "ltxattn_rotary_embed: %s's output repeats rows", name);
+  if (x.data == y.data && ((B > 1 && x.stride_b != y.stride_b) || (H > 1 && x.stride_h != y.stride_h) ||
+                           (T > 1 && x.stride_t != y.stride_t)))
+    return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_embed: %s in place needs the input's own strides", name);
+  return LTXATTN_OK;
+}
+
+}  // namespace
+}  // namespace ltx
+
+extern "C" {
+
+int ltxattn_rotary_frequencies(const ltxattn_rotary_frequency_args* a, double* frequencies, float* magnitude) {
+  using namespace ltx;
+  if (a == nullptr || frequencies == nullptr || magnitude == nullptr)
+    return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_frequencies: args, frequencies and magnitude are required");
+  if (a->rotary_dim < 2 || a->rotary_dim % 2)
+    return fail_rotary(LTXATTN_ERR_SHAPE, "ltxattn_rotary_frequencies: rotary_dim (%d) must be even and >= 2",
+                       a->rotary_dim);
+  if (a->scaling < LTXATTN_ROTARY_NONE || a->scaling > LTXATTN_ROTARY_BANDS)
+    return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_frequencies: unknown scaling %d", a->scaling);
+  const bool bands = a->scaling == LTXATTN_ROTARY_YARN || a->scaling == LTXATTN_ROTARY_BANDS;
+  if (!(a->theta > 0) || !std::isfinite(a->theta) || (a->scaling == LTXATTN_ROTARY_YARN && !(a->theta > 1)))
+    return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_frequencies: theta (%g) is out of range", a->theta);
+  if (a->scaling != LTXATTN_ROTARY_NONE && (!(a->factor > 0) || !std::isfinite(a->factor)))
+    return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_frequencies: factor (%g) must be positive", a->factor);
+  if (bands && (!(a->trained_length > 0) || !std::isfinite(a->trained_length) || !(a->slow > 0) ||
+                !(a->fast > a->slow) || !std::isfinite(a->fast)))
+    return fail_rotary(LTXATTN_ERR_ARG,
+                       "ltxattn_rotary_frequencies: trained_length must be positive and fast > slow > 0");
+  const int n = a->rotary_dim / 2;
+  const double two_pi = 6.283185307179586476925;
+  double theta = a->theta;
+  if (a->scaling == LTXATTN_ROTARY_NTK && n > 1) theta *= std::pow(a->factor, (double)n / (n - 1));
+  double low = 0, high = 0;
+  if (a->scaling == LTXATTN_ROTARY_YARN) {
+    // the pair that turns r times in L positions: theta^(-j / n) L = 2 pi r
+    auto pair_of = [&](double r) { return n * std::log(a->trained_length / (r * two_pi)) / std::log(theta); };
+    low = std::fmax(std::floor(pair_of(a->fast)), 0.0);
+    high = std::fmin(std::ceil(pair_of(a->slow)), (double)(a->rotary_dim - 1));
+  }
+  for (int j = 0; j < n; ++j) {
+    const double f = std::pow(theta, -(double)j / n);
+    double stretched = 0;  // the share of f / s
+    switch (a->scaling) {
+      case LTXATTN_ROTARY_LINEAR: stretched = 1; break;
+      case LTXATTN_ROTARY_YARN:
+        // an empty ramp is a step just above `low`
+        stretched = std::fmin(std::fmax((j - low) / std::fmax(high - low, 0.001), 0.0), 1.0);
+        break;
+      case LTXATTN_ROTARY_BANDS:
+        stretched = 1 - std::fmin(std::fmax((a->trained_length * f / two_pi - a->slow) / (a->fast - a->slow), 0.0), 1.0);
+        break;
+      default: break;
+    }
+    frequencies[j] = stretched == 0 ? f : f / a->factor * stretched + f * (1 - stretched);
+  }
+  *magnitude =
+      a->scaling == LTXATTN_ROTARY_YARN && a->factor > 1 ? (float)(0.1 * std::log(a->factor) + 1.0) : 1.0f;
+  return LTXATTN_OK;
+}
+
+int ltxattn_rotary_embed(const ltxattn_rotary_embed_args* a, void* stream) {
+  using namespace ltx;
+  if (a == nullptr) return fail_rotary(LTXATTN_ERR_ARG, "args is NULL");
+  if (a->dtype != LTXATTN_BF16 && a->dtype != LTXATTN_F32)
+    return fail_rotary(LTXATTN_ERR_DTYPE, "ltxattn_rotary_embed: dtype must be LTXATTN_BF16 or LTXATTN_F32");
+  if (a->batch < 0 || a->tokens < 0 || a->heads < 0 || a->kv_heads < 0 || a->head_dim < 1)
+    return fail_rotary(LTXATTN_ERR_SHAPE, "ltxattn_rotary_embed: a size is negative, or head_dim below 1");
+  if (a->rotary_dim < 2 || a->rotary_dim % 2 || a->rotary_dim > a->head_dim)
+    return fail_rotary(LTXATTN_ERR_SHAPE,
+                       "ltxattn_rotary_embed: rotary_dim (%d) must be even, >= 2 and at most head_dim (%d)",
+                       a->rotary_dim, a->head_dim);
+  if (a->layout != LTXATTN_ROTARY_HALF && a->layout != LTXATTN_ROTARY_INTERLEAVED)
+    return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_embed: unknown layout %d", a->layout);
+  if (a->positions != nullptr && a->position_bits != 64 && a->position_bits != 32)
+    return fail_rotary(LTXATTN_ERR_DTYPE, "ltxattn_rotary_embed: positions must be 64- or 32-bit integers");
+  const int64_t B = a->batch, T = a->tokens, H = a->heads, Hk = a->kv_heads;
+  if (H + Hk > 65535) return fail_rotary(LTXATTN_ERR_UNSUPPORTED, "ltxattn_rotary_embed: more than 65535 heads");
+  if (B == 0 || T == 0 || H + Hk == 0) return LTXATTN_OK;
+  if (a->frequencies == nullptr) return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_embed: frequencies is required");
+  if (reinterpret_cast<uintptr_t>(a->frequencies) % 8 ||
+      reinterpret_cast<uintptr_t>(a->positions) % (a->position_bits == 64 ? 8 : 4))
+    return fail_rotary(LTXATTN_ERR_ALIGN, "ltxattn_rotary_embed: frequencies or positions are not aligned to their type");
+  if (a->positions != nullptr && (a->position_stride_b < 0 || a->position_stride_t < 0))
+    return fail_rotary(LTXATTN_ERR_SHAPE, "ltxattn_rotary_embed: positions have a negative stride");
+  const bool bf16 = a->dtype == LTXATTN_BF16;
+  const int size = bf16 ? 2 : 4;
+  if (H > 0)
+    if (int rc = check_view("q", a->q, a->q_out, B, H, T, size)) return rc;
+  if (Hk > 0)
+    if (int rc = check_view("k", a->k, a->k_out, B, Hk, T, size)) return rc;
+
+  RotaryEmbedParams p{};
+  p.pairs = a->rotary_dim / 2;
+  // kP: the widest run (16 bytes at most) that the pairs, the part behind them and every row are multiples of
+  int kp = bf16 ? 8 : 4;
+  auto fits = [&](int n) {
+    if (p.pairs % n || a->head_dim % n) return false;
+    if (H > 0 && !(rows_aligned(a->q, B, H, T, n, size) && rows_aligned(a->q_out, B, H, T, n, size))) return false;
+    return Hk == 0 || (rows_aligned(a->k, B, Hk, T, n, size) && rows_aligned(a->k_out, B, Hk, T, n, size));
+  };
+  while (kp > 1 && !fits(kp)) kp /= 2;
+  const ltxattn_tensor* in[2] = {&a->q, &a->k};
+  const ltxattn_tensor* out[2] = {&a->q_out, &a->k_out};
+  bool in_place = true;
+  for (int i = 0; i < 2; ++i) {
+    p.v[i] = {in[i]->data,     out[i]->data,     in[i]->stride_b, in[i]->stride_h,
+              in[i]->stride_t, out[i]->stride_b, out[i]->stride_h, out[i]->stride_t};
+    if ((i == 0 ? H : Hk) > 0) in_place = in_place && in[i]->data == out[i]->data;
+  }
+  p.heads = (int)H;
+  p.total_heads = (int)(H + Hk);
+  p.T = (int)T;
+  p.turn_slots = p.pairs / kp;
+  p.slots = p.turn_slots + (in_place ? 0 : (a->head_dim - a->rotary_dim) / kp);
+  const int64_t items = B * T * p.slots;
+  if (items > 0x7fffffff - kRThreads)
+    return fail_rotary(LTXATTN_ERR_UNSUPPORTED, "ltxattn_rotary_embed: too many tokens for one call");
+  p.items = (unsigned)items;
+  p.freq = a->frequencies;
+  p.positions = a->positions;
+  p.pos64 = a->position_bits == 64;
+  p.pos_sb = a->position_stride_b;
+  p.pos_st = a->position_stride_t;
+  p.offset = a->offset;
+  p.magnitude = a->magnitude;
+  p.inverse = a->inverse != 0;
+  // heads per thread: as many as leave the GPU filled (the angles are then shared by more heads)
+  p.heads_per_thread = 32;
+  while (p.heads_per_thread > 1 &&
+         items * ((p.total_heads + p.heads_per_thread - 1) / p.heads_per_thread) < 148 * 1024)
+    p.heads_per_thread /= 2;
+  const dim3 grid((unsigned)((items + kRThreads - 1) / kRThreads),
+                  (unsigned)((p.total_heads + p.heads_per_thread - 1) / p.heads_per_thread));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool il = a->layout == LTXATTN_ROTARY_INTERLEAVED;
+  if (bf16) {
+    switch (kp) {
+      case 8: launch<__nv_bfloat16, 8>(p, il, grid, st); break;
+      case 4: launch<__nv_bfloat16, 4>(p, il, grid, st); break;
+      case 2: launch<__nv_bfloat16, 2>(p, il, grid, st); break;
+      default: launch<__nv_bfloat16, 1>(p, il, grid, st); break;
+    }
+  } else {
+    switch (kp) {
+      case 4: launch<float, 4>(p, il, grid, st); break;
+      case 2: launch<float, 2>(p, il, grid, st); break;
+      default: launch<float, 1>(p, il, grid, st); break;
+    }
+  }
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail_rotary(LTXATTN_ERR_CUDA, "ltxattn_rotary_embed: %s", cudaGetErrorString(e));
+  return LTXATTN_OK;
+}
+
+}  // extern "C"

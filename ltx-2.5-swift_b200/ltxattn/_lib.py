@@ -30,7 +30,8 @@ EXPORTED = (
     "ltxattn_comm_size", "ltxattn_selftest_wait_timeout", "ltxattn_memory_plan",
     "ltxattn_linear", "ltxattn_linear_workspace", "ltxattn_head_gate",
     "ltxattn_out_project_workspace", "ltxattn_out_project_allreduce", "ltxattn_fwd_gather",
-    "ltxattn_out_project_fused",
+    "ltxattn_out_project_fused", "ltxattn_rotary_frequencies", "ltxattn_rotary_embed",
+    "ltxattn_gated_ffn", "ltxattn_gated_ffn_workspace", "ltxattn_gated_ffn_bwd", "ltxattn_gated_ffn_bwd_workspace",
 )
 
 
@@ -163,6 +164,40 @@ class MemoryPlanInfo(ctypes.Structure):
                 ("fits", ctypes.c_int32), ("bytes_per_token", ctypes.c_double)]
 
 
+class RotaryFrequencyArgs(ctypes.Structure):
+    _fields_ = [("rotary_dim", ctypes.c_int32), ("scaling", ctypes.c_int32), ("theta", ctypes.c_double),
+                ("factor", ctypes.c_double), ("trained_length", ctypes.c_double), ("fast", ctypes.c_double),
+                ("slow", ctypes.c_double)]
+
+
+class RotaryEmbedArgs(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("rotary_dim", ctypes.c_int32), ("layout", ctypes.c_int32), ("inverse", ctypes.c_int32),
+                ("magnitude", ctypes.c_float), ("q", Tensor), ("q_out", Tensor), ("k", Tensor), ("k_out", Tensor),
+                ("frequencies", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("position_bits", ctypes.c_int32),
+                ("position_stride_b", ctypes.c_int64), ("position_stride_t", ctypes.c_int64),
+                ("offset", ctypes.c_int64)]
+
+
+def _rows(*names):
+    return [f for n in names for f in ((n, ctypes.c_void_p), (n + "_stride", ctypes.c_int64))]
+
+
+_FFN_SIZES = [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("m", ctypes.c_int32),
+              ("hidden", ctypes.c_int32), ("inner", ctypes.c_int32), ("out_dim", ctypes.c_int32)]
+_WORKSPACE = [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class GatedFfnArgs(ctypes.Structure):
+    _fields_ = _FFN_SIZES + _rows("x", "w_gate", "w_up", "w_down", "out", "gate", "up") + _WORKSPACE
+
+
+class GatedFfnBwdArgs(ctypes.Structure):
+    _fields_ = _FFN_SIZES + _rows("x", "w_gate", "w_up", "w_down", "gate", "up", "dout", "dx", "dw_gate", "dw_up",
+                                  "dw_down") + _WORKSPACE
+
+
 def load(path: str = LIB_PATH):
     """Load the in-tree library; raises when it has not been built."""
     global _lib
@@ -231,6 +266,16 @@ def load(path: str = LIB_PATH):
     L.ltxattn_out_project_workspace.restype = ctypes.c_size_t
     L.ltxattn_out_project_allreduce.argtypes = [ctypes.POINTER(OutProjectArgs), vp, vp]
     L.ltxattn_out_project_allreduce.restype = ctypes.c_int
+    L.ltxattn_rotary_frequencies.argtypes = [ctypes.POINTER(RotaryFrequencyArgs), ctypes.POINTER(ctypes.c_double),
+                                             ctypes.POINTER(ctypes.c_float)]
+    L.ltxattn_rotary_frequencies.restype = ctypes.c_int
+    L.ltxattn_rotary_embed.argtypes = [ctypes.POINTER(RotaryEmbedArgs), vp]
+    L.ltxattn_rotary_embed.restype = ctypes.c_int
+    for name, args in (("ltxattn_gated_ffn", GatedFfnArgs), ("ltxattn_gated_ffn_bwd", GatedFfnBwdArgs)):
+        getattr(L, name).argtypes = [ctypes.POINTER(args), vp]
+        getattr(L, name).restype = ctypes.c_int
+        getattr(L, name + "_workspace").argtypes = [ctypes.POINTER(args)]
+        getattr(L, name + "_workspace").restype = ctypes.c_size_t
     L.ltxattn_abi_version.argtypes = []
     L.ltxattn_abi_version.restype = ctypes.c_int
     _lib = L

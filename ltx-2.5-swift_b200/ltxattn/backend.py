@@ -136,6 +136,33 @@ def _stream_ptr(stream) -> int:
     return s.cuda_stream
 
 
+class _on:
+    """Runs a call on the tensors' device and on ``stream`` (torch's current one
+    there if None): what is allocated inside belongs to that stream.  Gives the
+    stream's handle."""
+
+    __slots__ = ("device", "stream", "guard")
+
+    def __init__(self, device: torch.device, stream):
+        if stream is not None and stream.device != device:
+            raise Failure("arg", f"the stream is on {stream.device}, the tensors on {device}", _lib.ERR_ARG)
+        self.device, self.stream, self.guard = device, stream, None
+
+    def __enter__(self):
+        if self.stream is not None:
+            self.guard = torch.cuda.stream(self.stream)
+        elif torch.cuda.current_device() != self.device.index:
+            self.guard = torch.cuda.device(self.device)
+        if self.guard is not None:
+            self.guard.__enter__()
+        return ctypes.c_void_p(_stream_ptr(self.stream))
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
 class AttentionBackend:
     """The attention seam, backed by libltxattn_cuda."""
 
