@@ -19,18 +19,19 @@ from .backend import Failure, _check_cuda, _on
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1, "gelu": 2}
 
 
-def _matrix(name: str, t: torch.Tensor, rows: int, cols: int, device) -> tuple:
-    """(address, row stride) of a bf16 [rows, cols] matrix."""
+def _matrix(name: str, t: torch.Tensor, rows: int, cols: int, device: int) -> tuple:
+    """(address, row stride) of a bf16 [rows, cols] matrix on that device."""
     _check_cuda(name, t)
     if t.dtype != torch.bfloat16:
         raise Failure("dtype", f"{name} must be bfloat16", _lib.ERR_DTYPE)
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+    if t.shape != (rows, cols):
         raise Failure.shape(name, t.shape, f"[{rows}, {cols}]")
-    if t.device != device:
-        raise Failure("arg", f"{name} is on {t.device}, x on {device}", _lib.ERR_ARG)
-    if t.stride(1) != 1 and cols > 1:
+    if t.get_device() != device:
+        raise Failure("arg", f"{name} is on {t.device}, the tokens on cuda:{device}", _lib.ERR_ARG)
+    stride, unit = t.stride()
+    if unit != 1 and cols > 1:
         raise Failure("align", f"{name} must have a unit stride along its last dim", _lib.ERR_ALIGN)
-    return t.data_ptr(), t.stride(0) if rows > 1 else cols
+    return t.data_ptr(), stride if rows > 1 else cols
 
 
 def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -44,13 +45,17 @@ def _activation(name: str) -> int:
     return ACTIVATIONS[name]
 
 
-def _output(name: str, t: Optional[torch.Tensor], shape, device):
-    """An output of that shape as the caller gave it (it must be one that can be written as rows) or a new one."""
+def _output(name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor):
+    """An output of that shape: the caller's, or a new one on the device of ``like``."""
     if t is None:
-        return torch.empty(shape, dtype=torch.bfloat16, device=device)
-    if tuple(t.shape) != tuple(shape):
+        return like.new_empty(shape, dtype=torch.bfloat16)
+    if t.shape != tuple(shape):
         raise Failure.shape(name, t.shape, str(list(shape)))
     return t
+
+
+def _workspace(need: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    return like.new_empty((need,), dtype=torch.uint8) if need else None
 
 
 def _out_rows(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -75,7 +80,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     _check_cuda("x", x)
     if x.dim() < 1:
         raise Failure.shape("x", x.shape, "[..., hidden]")
-    device = x.device
+    device = x.get_device()
     for name, w in (("w_gate", w_gate), ("w_down", w_down)):
         if not isinstance(w, torch.Tensor) or w.dim() != 2:
             raise Failure.shape(name, getattr(w, "shape", ()), "a matrix")
@@ -84,7 +89,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     with _on(device, stream) as st:
         x2 = _rows("x", x)
         m, hidden = x2.shape
-        y = _output("out", out, lead + (out_dim,), device)
+        y = _output("out", out, lead + (out_dim,), x)
         a = _lib.GatedFfnArgs(_lib.BF16, act, m, hidden, inner, out_dim, *_matrix("x", x2, m, hidden, device),
                               *_matrix("w_gate", w_gate, inner, hidden, device),
                               *_matrix("w_up", w_up, inner, hidden, device),
@@ -92,13 +97,13 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
                               *_matrix("out", _out_rows("out", y), m, out_dim, device))
         gate = up = None
         if save:
-            gate = torch.empty(lead + (inner,), dtype=torch.bfloat16, device=device)
+            gate = x.new_empty(lead + (inner,))
             up = torch.empty_like(gate)
             a.gate, a.gate_stride, a.up, a.up_stride = gate.data_ptr(), inner, up.data_ptr(), inner
         L = _lib.load()
-        need = int(L.ltxattn_gated_ffn_workspace(ctypes.byref(a)))
-        if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=device)
+        need = L.ltxattn_gated_ffn_workspace(ctypes.byref(a))
+        ws = _workspace(need, x)
+        if ws is not None:
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
         rc = L.ltxattn_gated_ffn(ctypes.byref(a), st)
     if rc != _lib.OK:
@@ -122,7 +127,7 @@ def gated_ffn_backward(x: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: to
     _check_cuda("dout", dout)
     if dout.dim() < 1:
         raise Failure.shape("dout", dout.shape, "[..., out]")
-    device = dout.device
+    device = dout.get_device()
     if not isinstance(w_gate, torch.Tensor) or w_gate.dim() != 2:
         raise Failure.shape("w_gate", getattr(w_gate, "shape", ()), "a matrix")
     inner, hidden = w_gate.shape
@@ -154,23 +159,23 @@ def gated_ffn_backward(x: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: to
         put("up", _rows("up", up), m, inner)
         put("dout", d2, m, out_dim)
         if need_dx:
-            dx = _output("dx", dx, tuple(lead) + (hidden,), device)
+            dx = _output("dx", dx, tuple(lead) + (hidden,), dout)
             put("dx", _out_rows("dx", dx), m, hidden)
         else:
             dx = None
         if need_dw:
-            dw_gate = _output("dw_gate", dw_gate, (inner, hidden), device)
-            dw_up = _output("dw_up", dw_up, (inner, hidden), device)
-            dw_down = _output("dw_down", dw_down, (out_dim, inner), device)
+            dw_gate = _output("dw_gate", dw_gate, (inner, hidden), dout)
+            dw_up = _output("dw_up", dw_up, (inner, hidden), dout)
+            dw_down = _output("dw_down", dw_down, (out_dim, inner), dout)
             put("dw_gate", dw_gate, inner, hidden)
             put("dw_up", dw_up, inner, hidden)
             put("dw_down", dw_down, out_dim, inner)
         else:
             dw_gate = dw_up = dw_down = None
         L = _lib.load()
-        need = int(L.ltxattn_gated_ffn_bwd_workspace(ctypes.byref(a)))
-        if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=device)
+        need = L.ltxattn_gated_ffn_bwd_workspace(ctypes.byref(a))
+        ws = _workspace(need, dout)
+        if ws is not None:
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
         rc = L.ltxattn_gated_ffn_bwd(ctypes.byref(a), st)
     if rc != _lib.OK:

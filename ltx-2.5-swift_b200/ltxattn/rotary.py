@@ -19,7 +19,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .backend import Failure, _check_cuda, _dtype_code, _view, _on
+from .backend import Failure, _check_cuda, _dtype_code, _on
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
@@ -49,61 +49,72 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str = "
     return torch.tensor(list(out), dtype=torch.float64).to(device), magnitude.value
 
 
+def _heads(name: str, t: torch.Tensor, shape: tuple, dtype, device: int) -> _lib.Tensor:
+    """The view of a [B, heads, tokens, D] tensor on that device."""
+    _check_cuda(name, t)
+    if t.shape != shape:
+        raise Failure.shape(name, t.shape, str(list(shape)))
+    if t.dtype != dtype:
+        raise Failure("dtype", f"{name} is {t.dtype}, q is {dtype}", _lib.ERR_DTYPE)
+    _same_device(name, t, device)
+    sb, sh, st, sd = t.stride()
+    if sd != 1:
+        raise Failure("align", f"{name} must have a unit stride in its last dim", _lib.ERR_ALIGN)
+    return _lib.Tensor(t.data_ptr(), sb, sh, st)
+
+
+def _same_device(name: str, t: torch.Tensor, device: int):
+    if t.get_device() != device:
+        raise Failure("arg", f"{name} is on {t.device}, q on cuda:{device}", _lib.ERR_ARG)
+
+
 def _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k, stream, inverse):
     _check_cuda("q", q)
     if q.dim() != 4:
         raise Failure.shape("q", q.shape, "[B, heads, tokens, headDim]")
-    B, H, T, D = q.shape
-    device = q.device
+    shape, dtype, device = q.shape, q.dtype, q.get_device()
+    B, H, T, D = shape
     if layout not in LAYOUTS:
         raise Failure("arg", f"layout {layout!r} is neither 'half' nor 'interleaved'", _lib.ERR_ARG)
     _check_cuda("frequencies", frequencies)
+    _same_device("frequencies", frequencies, device)
     if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
         raise Failure.shape("frequencies", frequencies.shape, "[rotaryDim / 2] float64, contiguous")
-    Hk = 0
-    tensors = [frequencies]
+    a = _lib.RotaryEmbedArgs(_dtype_code(q), B, T, H, 0, D, 2 * frequencies.shape[0], LAYOUTS[layout],
+                             1 if inverse else 0, magnitude)
+    a.frequencies, a.offset = frequencies.data_ptr(), offset
+    a.q = _heads("q", q, shape, dtype, device)
     if k is not None:
-        _check_cuda("k", k)
-        if k.dim() != 4 or k.shape[0] != B or k.shape[2] != T or k.shape[3] != D:
+        if k.dim() != 4:
             raise Failure.shape("k", k.shape, f"[{B}, kvHeads, {T}, {D}]")
-        if k.dtype != q.dtype:
-            raise Failure("dtype", "q and k must share one dtype", _lib.ERR_DTYPE)
-        Hk = k.shape[1]
-        tensors.append(k)
-    pos_ptr, pos_bits, pos_sb, pos_st = None, 0, 0, 0
+        k_shape = (B, k.shape[1], T, D)
+        a.kv_heads, a.k = k_shape[1], _heads("k", k, k_shape, dtype, device)
+    elif out_k is not None:
+        raise Failure("arg", "out_k without k", _lib.ERR_ARG)
     if positions is not None:
         _check_cuda("positions", positions)
-        if positions.dtype not in (torch.int64, torch.int32):
-            raise Failure("dtype", f"positions are {positions.dtype}, expected int64 or int32", _lib.ERR_DTYPE)
-        shape = tuple(positions.shape)
-        if shape not in ((T,), (1, T), (B, T)):
-            raise Failure.shape("positions", shape, f"[{T}] or [1|{B}, {T}]")
-        pos_ptr, pos_bits, pos_st = positions.data_ptr(), 8 * positions.element_size(), positions.stride(-1)
-        pos_sb = positions.stride(0) if len(shape) == 2 and shape[0] > 1 else 0
-        tensors.append(positions)
-    for name, o, x in (("out_q", out_q, q), ("out_k", out_k, k)):
-        if o is not None:
-            if x is None:
-                raise Failure("arg", f"{name} without its input", _lib.ERR_ARG)
-            _check_cuda(name, o)
-            if o.dtype != x.dtype:
-                raise Failure("dtype", f"{name} must have the dtype of its input", _lib.ERR_DTYPE)
-            tensors.append(o)
-    for t in tensors:
-        if t.device != device:
-            raise Failure("arg", f"q is on {device}, another tensor on {t.device}", _lib.ERR_ARG)
-    with _on(device, stream) as st:
-        out_q = torch.empty_like(q) if out_q is None else out_q
-        none = _lib.Tensor()
-        if k is not None:
-            out_k = torch.empty_like(k) if out_k is None else out_k
-            vk, vok = _view("k", k, (B, Hk, T, D)), _view("out_k", out_k, (B, Hk, T, D))
+        _same_device("positions", positions, device)
+        if positions.dtype == torch.int64:
+            a.position_bits = 64
+        elif positions.dtype == torch.int32:
+            a.position_bits = 32
         else:
-            vk = vok = none
-        a = _lib.RotaryEmbedArgs(_dtype_code(q), B, T, H, Hk, D, 2 * frequencies.shape[0], LAYOUTS[layout],
-                                 1 if inverse else 0, magnitude, _view("q", q, (B, H, T, D)),
-                                 _view("out_q", out_q, (B, H, T, D)), vk, vok, frequencies.data_ptr(), pos_ptr,
-                                 pos_bits, pos_sb, pos_st, offset)
+            raise Failure("dtype", f"positions are {positions.dtype}, expected int64 or int32", _lib.ERR_DTYPE)
+        p_shape = tuple(positions.shape)
+        if p_shape != (B, T) and p_shape != (T,) and p_shape != (1, T):
+            raise Failure.shape("positions", p_shape, f"[{T}] or [1|{B}, {T}]")
+        strides = positions.stride()
+        a.positions, a.position_stride_t = positions.data_ptr(), strides[-1]
+        if len(p_shape) == 2 and p_shape[0] > 1:
+            a.position_stride_b = strides[0]
+    with _on(device, stream) as st:
+        if out_q is None:
+            out_q = torch.empty_like(q)
+        a.q_out = _heads("out_q", out_q, shape, dtype, device)
+        if k is not None:
+            if out_k is None:
+                out_k = torch.empty_like(k)
+            a.k_out = _heads("out_k", out_k, k_shape, dtype, device)
         rc = _lib.load().ltxattn_rotary_embed(ctypes.byref(a), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)

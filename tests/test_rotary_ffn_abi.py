@@ -139,7 +139,7 @@ def rotary_args(**kw):
     (dict(positions=4096, position_bits=16), _lib.ERR_DTYPE),
     (dict(positions=4100), _lib.ERR_ALIGN),
     (dict(positions=4096, position_stride_t=-1), _lib.ERR_SHAPE),
-    (dict(heads=65535), _lib.ERR_UNSUPPORTED),
+    (dict(head_dim=16384, rotary_dim=16384), _lib.ERR_UNSUPPORTED),
     (dict(tokens=2 ** 30), _lib.ERR_UNSUPPORTED),
     ({"q.data": None}, _lib.ERR_ARG),
     ({"k_out.data": None}, _lib.ERR_ARG),
