@@ -1,0 +1,118 @@
+// ffn_common.cuh -- what the two kernels of the gated feed-forward block share:
+// the activations and the TMA maps.
+#pragma once
+
+#include <cstdio>
+#include <mutex>
+
+#include "../../include/ltxattn.h"
+#include "ltxattn_internal.h"
+#include "sm100.cuh"
+
+namespace ltx {
+
+// ---------------------------------------------------------------------------
+// activations (fp32)
+
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
+
+// act(g), and with kSlope its derivative too.
+template <bool kSlope>
+__device__ __forceinline__ float activate(int kind, float g, float& slope) {
+  if (kind == LTXATTN_SILU) {
+    const float s = sigmoid(g);
+    if (kSlope) slope = s * fmaf(g, 1.0f - s, 1.0f);
+    return g * s;
+  }
+  if (kind == LTXATTN_GELU_TANH) {
+    // (1 + tanh z) / 2 = sigmoid(2 z)
+    constexpr float c2 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+    const float g2 = g * g;
+    const float s = sigmoid(c2 * g * fmaf(0.044715f, g2, 1.0f));
+    if (kSlope) {
+      const float t = g * s * (1.0f - s);  // 0 far out, where g2 may be infinite
+      slope = t == 0.0f ? s : fmaf(t, c2 * fmaf(0.134145f, g2, 1.0f), s);
+    }
+    return g * s;
+  }
+  const float s = 0.5f * erfcf(-0.70710678118654752f * g);
+  if (kSlope) slope = fmaf(g, 0.3989422804014327f * __expf(-0.5f * g * g), s);
+  return g * s;
+}
+
+__device__ __forceinline__ float lo_f(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float hi_f(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// The gradient through act(g) * u from dh: (dg, du), and the product itself.
+__device__ __forceinline__ void slopes(int kind, float g, float u, float dh, float& dg, float& du, float& h) {
+  float slope;
+  const float a = activate<true>(kind, g, slope);
+  dg = dh * u * slope;
+  du = dh * a;
+  h = a * u;
+}
+
+// 8 consecutive bf16 of a row (16-byte aligned).
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                                            pack_bf16x2(v[6], v[7]));
+}
+
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 w = *reinterpret_cast<const uint4*>(p);
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[2 * e] = lo_f(u[e]);
+    v[2 * e + 1] = hi_f(u[e]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+
+// Records the message and gives the status back.
+int fail_ffn(int status, const char* fmt, ...);
+
+// bf16 [rows, cols], `stride` elements between rows; boxes of 64 columns (one swizzle row) and box_rows rows.
+int ffn_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t stride, int box_rows, const char* name);
+
+constexpr int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int kFfnK = 64;  // K per pipeline stage: one 128-byte swizzle row of bf16
+
+// One product of the block for few tokens (ffn_narrow_sm100.cu): the weights'
+// rows or columns are the rows of the accumulator, the tokens its columns.
+struct NarrowParams {
+  CUtensorMap a[2];  // weights (kNarrowProduct: gate and up; else K slices from kb_first on come from the second pair)
+  CUtensorMap b[2];  // tokens
+  int tokens, features;
+  int kb, kb_first;      // 64-wide K slices in all, and of the first pair
+  int columns;           // tokens of a tile: a multiple of 16, the box of b
+  int tiles;             // feature tiles
+  int stages;
+  int activation;
+  __nv_bfloat16* out;    // [tokens, features]
+  int64_t out_stride;
+  __nv_bfloat16 *gate, *up, *dgate, *dup;  // as GemmParams
+  int64_t gate_stride, up_stride, dgate_stride, dup_stride;
+  int* err;
+};
+
+enum NarrowMode {
+  kNarrowProduct,  // out = act(x Wg^T) * (x Wu^T), weights K-major
+  kNarrowStore,    // out = h Wd^T, weights K-major
+  kNarrowSlopes,   // dh = dout Wd and what follows from it, weights MN-major
+  kNarrowStoreMN   // dx = dg Wg + du Wu, weights MN-major
+};
+
+constexpr int kNarrowColumns = 128;  // tokens of a tile at most
+
+// Tokens of a tile for a call of that many.
+inline int narrow_columns(int tokens) { return tokens >= kNarrowColumns ? kNarrowColumns : (int)div_up(tokens, 16) * 16; }
+// Rows of the boxes of a[]: 128 features K-major, 64 of K MN-major.
+inline int narrow_box(NarrowMode mode) { return mode == kNarrowProduct || mode == kNarrowStore ? 128 : kFfnK; }
+// `follows`: the kernel reads what the one before it in the stream wrote, and may start while that one ends.
+int launch_narrow(NarrowMode mode, NarrowParams& p, bool follows, const char* call, cudaStream_t st);
+
+}  // namespace ltx

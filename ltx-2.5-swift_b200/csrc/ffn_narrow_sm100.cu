@@ -1,0 +1,361 @@
+// ffn_narrow_sm100.cu -- the products of the gated feed-forward block for few
+// tokens (one to some hundreds), on tcgen05 (sm_100a).
+//
+// With few tokens a product reads every weight once and uses it a few times: it
+// is bound by the weights' bytes (402 MB for one token at 4096 x 16384), and
+// the work is to keep all SMs loading.  So the roles are swapped: a tile is 128
+// features, whose weights are the MMA's A operand, by up to 128 tokens as its
+// B operand (N = the tokens, rounded up to 16).  No weight row is loaded for a
+// token that is not there, and the epilogue has a thread per feature instead of
+// one per token.
+//
+// Tiles are few (4096 features: 32), so a cluster of 1 to 8 CTAs shares a
+// tile: each takes a part of K, leaves its fp32 partial in its own shared
+// memory, and after a cluster barrier the CTAs add the parts of a share of the
+// tokens each, in rank order, and finish those (the sums do not depend on which
+// CTA came first).
+//
+// The kernel that follows another (the second product of a call) starts while
+// that one ends: its weights do not depend on it, so the first stages are loaded
+// before it waits for the other's output.
+#include <algorithm>
+
+#include "ffn_common.cuh"
+
+namespace ltx {
+
+namespace {
+
+constexpr int kNThreads = 384;  // 4 control warps, 8 epilogue warps
+constexpr int kNRows = 128;     // features of a tile (UMMA M)
+constexpr int kNMaxStages = 12;
+constexpr int kNMaxCluster = 8;
+constexpr uint32_t kNATile = kNRows * kFfnK * 2;
+constexpr uint32_t kNChunk = 64 * kFfnK * 2;  // MN-major: 64 features x 64 rows of K
+constexpr uint32_t kNStageSpace = 216 * 1024;
+// full, empty per stage, acc_full
+constexpr uint32_t kNOffBar = kNStageSpace;
+constexpr uint32_t kNOffCtl = kNOffBar + (2 * kNMaxStages + 1) * 8;
+constexpr uint32_t kNSmem = kNOffCtl + 16 + 1024;  // + alignment slack
+static_assert(kNSmem <= kMaxDynamicSmem, "shared memory of a CTA");
+// a tile's partial sums, [accumulator column][128 features] fp32, take the stages' place
+static_assert(2 * kNarrowColumns * kNRows * 4 <= kNStageSpace, "partial sums");
+
+// bytes of the weights in a stage
+template <NarrowMode kMode>
+constexpr uint32_t kWeights = kMode == kNarrowProduct ? 2 * kNATile : kNATile;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+// Every thread of every CTA of the cluster comes here, whatever happened before:
+// a CTA whose wait gave up still arrives.  Shared memory written before is
+// visible to the cluster after.
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// 4 floats at the address that `local` has in this CTA, of the CTA with that rank.
+__device__ __forceinline__ float4 peer_load4(uint32_t local, uint32_t rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+
+// The sum over the cluster's parts of 8 features (from `feature`) of one accumulator column.
+__device__ __forceinline__ void sum8(uint32_t partial, int column, int feature, uint32_t ranks, float (&v)[8]) {
+  const uint32_t at = partial + (column * kNRows + feature) * 4;
+  for (uint32_t r = 0; r < ranks; ++r) {
+    const float4 a = peer_load4(at, r), b = peer_load4(at + 16, r);
+    const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = r == 0 ? w[e] : v[e] + w[e];
+  }
+}
+
+template <NarrowMode kMode>
+__global__ void __launch_bounds__(kNThreads, 1) narrow_kernel(const __grid_constant__ NarrowParams p) {
+  constexpr bool kDual = kMode == kNarrowProduct;
+  constexpr bool kAMN = kMode == kNarrowSlopes || kMode == kNarrowStoreMN;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = align1024(smem_raw);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + kNOffBar);
+  uint64_t* empty = full + kNMaxStages;
+  uint64_t* acc_full = empty + kNMaxStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + kNOffCtl);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + kNOffCtl + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const int tile = blockIdx.x / ranks;
+  const int f0 = (tile % p.tiles) * kNRows;
+  const int t0 = (tile / p.tiles) * p.columns;
+  const int kb0 = (int)((int64_t)p.kb * rank / ranks), kb1 = (int)((int64_t)p.kb * (rank + 1) / ranks);
+  const int kb_n = kb1 - kb0;  // >= 1: there are no more ranks than K slices
+  const uint32_t stage_bytes = kWeights<kMode> + p.columns * kFfnK * 2;
+  const int stages = p.stages;
+  const int acc_columns = kDual ? 2 * p.columns : p.columns;
+  uint32_t tmem_columns = 32;
+  while ((int)tmem_columns < acc_columns) tmem_columns *= 2;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, tmem_columns);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dep_launch_dependents();
+
+  if (warp == 0 && lane == 0) {
+    auto weights = [&](int i) {
+      const int st = i % stages, kb = kb0 + i;
+      uint8_t* sa = sm + st * stage_bytes;
+      mbar_arrive_expect_tx(full + st, stage_bytes);
+      const int part = kb >= p.kb_first;
+      const int k0 = (part ? kb - p.kb_first : kb) * kFfnK;
+      if (kAMN) {
+#pragma unroll
+        for (int c = 0; c < kNRows / 64; ++c) tma_load_2d(&p.a[part], full + st, sa + c * kNChunk, f0 + c * 64, k0);
+      } else if (kDual) {
+        tma_load_2d(&p.a[0], full + st, sa, k0, f0);
+        tma_load_2d(&p.a[1], full + st, sa + kNATile, k0, f0);
+      } else {
+        tma_load_2d(&p.a[0], full + st, sa, k0, f0);
+      }
+    };
+    auto tokens = [&](int i) {
+      const int st = i % stages, kb = kb0 + i;
+      const int part = kb >= p.kb_first;
+      const int k0 = (part ? kb - p.kb_first : kb) * kFfnK;
+      tma_load_2d(&p.b[part], full + st, sm + st * stage_bytes + kWeights<kMode>, k0, t0);
+    };
+    const int first = min(stages, kb_n);
+    for (int i = 0; i < first; ++i) weights(i);
+    grid_dep_wait();  // what the tokens' operand is read from is written by the kernel before
+    for (int i = 0; i < first; ++i) tokens(i);
+    int i = first;
+    for (; i < kb_n; ++i) {
+      if (!mbar_wait(empty + i % stages, (i / stages - 1) & 1, abort_flag, p.err, 65)) break;
+      weights(i);
+      tokens(i);
+    }
+    // never leave the CTA with a bulk copy still writing its shared memory
+    for (int j = i < stages ? 0 : i - stages; j < i; ++j) drain_wait(full + j % stages, (j / stages) & 1);
+  } else if (warp == 1 && lane == 0) {
+    const uint32_t idesc = idesc_bf16_f32(kNRows, p.columns, kAMN, 0);
+    const SDesc a0 = sdesc_split(smem_u32(sm), kAMN ? kNChunk : 16, 1024);
+    const SDesc b0 = sdesc_split(smem_u32(sm) + kWeights<kMode>, 16, 1024);
+    // 16 of K further along: 32 bytes of each row K-major, 16 rows of 128 bytes MN-major
+    constexpr uint32_t a_step = kAMN ? 128 : 2;
+    for (int i = 0; i < kb_n; ++i) {
+      const int st = i % stages;
+      if (!mbar_wait(full + st, (i / stages) & 1, abort_flag, p.err, 66)) break;
+      tc_fence_after();
+      const uint32_t alo = a0.lo + st * (stage_bytes >> 4), blo = b0.lo + st * (stage_bytes >> 4);
+#pragma unroll
+      for (int kk = 0; kk < kFfnK / 16; ++kk) {
+        const uint32_t more = (i > 0 || kk > 0) ? 1u : 0u;
+        umma_ss2(tmem, alo + kk * a_step, a0.hi, blo + kk * 2, b0.hi, idesc, more);
+        if (kDual)
+          umma_ss2(tmem + p.columns, alo + (kNATile >> 4) + kk * a_step, a0.hi, blo + kk * 2, b0.hi, idesc, more);
+      }
+      umma_commit(empty + st);  // the stage is free once these MMAs have read it
+    }
+    umma_commit(acc_full);
+    drain_wait(acc_full, 0);  // no MMA still running when the CTA tears down
+  }
+  __syncwarp();
+
+  // this CTA's partial sums, where the stages were: acc_full comes after the last MMA's reads, and every
+  // copy has landed before an MMA that read it
+  const uint32_t partial = smem_u32(sm);
+  if (warp >= 4) {
+    const bool have = warp_wait(acc_full, 0, abort_flag, p.err, 67);
+    tc_fence_after();
+    const int quadrant = warp & 3;
+    float* row = reinterpret_cast<float*>(sm) + quadrant * 32 + lane;
+    if (have) {
+      for (int c = ((warp - 4) >> 2) * 16; c < acc_columns; c += 32) {
+        __syncwarp();
+        uint32_t r[16];
+        tmem_ld16(tmem + (static_cast<uint32_t>(quadrant * 32) << 16) + c, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) row[(c + e) * kNRows] = __uint_as_float(r[e]);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_barrier();
+
+  // the cluster's CTAs share the tile's tokens; a thread finishes 8 features of one
+  const int n_tokens = min(p.columns, p.tokens - t0);
+  const int first = (int)(n_tokens * rank / ranks), last = (int)(n_tokens * (rank + 1) / ranks);
+  if (warp >= 4 && *abort_flag == 0) {
+    const int i = threadIdx.x - 128;
+    const int col = f0 + (i % 16) * 8;
+    for (int t = first + i / 16; t < last; t += 16) {
+      if (col >= p.features) break;
+      const int64_t token = t0 + t;
+      float v[8];
+      sum8(partial, t, (i % 16) * 8, ranks, v);
+      if (kDual) {
+        float u[8];
+        sum8(partial, p.columns + t, (i % 16) * 8, ranks, u);
+        if (p.gate != nullptr) {
+          store8(p.gate + token * p.gate_stride + col, v);
+          store8(p.up + token * p.up_stride + col, u);
+        }
+        float unused;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = activate<false>(p.activation, v[e], unused) * u[e];
+      }
+      if (kMode == kNarrowSlopes) {
+        float g[8], u[8], dg[8], du[8];
+        load8(p.gate + token * p.gate_stride + col, g);
+        load8(p.up + token * p.up_stride + col, u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) slopes(p.activation, g[e], u[e], v[e], dg[e], du[e], v[e]);
+        store8(p.dgate + token * p.dgate_stride + col, dg);
+        store8(p.dup + token * p.dup_stride + col, du);
+        if (p.out == nullptr) continue;  // h is wanted for dw_down alone
+      }
+      store8(p.out + token * p.out_stride + col, v);
+    }
+  }
+  __syncthreads();
+  cluster_barrier();  // no CTA leaves while another reads its partial sums
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_columns);
+  }
+}
+
+constexpr int kMaxDev = 64;
+std::mutex g_mu;
+
+struct Occupancy {
+  bool ready;
+  int clusters[kNMaxCluster + 1];  // clusters of that size that run together
+};
+Occupancy g_occupancy[kMaxDev][4];
+
+template <NarrowMode kMode>
+cudaError_t prepare(Occupancy* out) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDev) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(g_mu);
+  Occupancy& o = g_occupancy[dev][kMode];
+  if (!o.ready) {
+    e = cudaFuncSetAttribute(narrow_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem);
+    if (e != cudaSuccess) return e;
+    for (int s = 1; s <= kNMaxCluster; ++s) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = s * 64;
+      cfg.blockDim = kNThreads;
+      cfg.dynamicSmemBytes = kNSmem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = s;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&o.clusters[s], narrow_kernel<kMode>, &cfg);
+      if (e != cudaSuccess) return e;
+    }
+    o.ready = true;
+  }
+  *out = o;
+  return cudaSuccess;
+}
+
+// CTAs that share a tile: the size that ends first, counting rounds of clusters
+// over the SMs, K slices of a CTA, and what a round costs besides (about four
+// slices: filling the pipeline, the exchange, the epilogue).
+int choose_cluster(const Occupancy& o, int64_t tiles, int kb) {
+  int best = 1;
+  int64_t best_cost = -1;
+  for (int s = 1; s <= std::min(kNMaxCluster, kb); ++s) {
+    if (o.clusters[s] < 1) continue;
+    const int64_t cost = div_up(tiles, o.clusters[s]) * (div_up(kb, s) + 4);
+    if (best_cost < 0 || cost < best_cost) {
+      best = s;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
+template <NarrowMode kMode>
+int launch(NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
+  Occupancy o;
+  cudaError_t e = prepare<kMode>(&o);
+  if (e == cudaSuccess) {
+    const int64_t tiles = (int64_t)p.tiles * div_up(p.tokens, p.columns);
+    const int cluster = choose_cluster(o, tiles, p.kb);
+    if (tiles * cluster > 0x7fffffff) return fail_ffn(LTXATTN_ERR_UNSUPPORTED, "%s: too many output tiles", call);
+    p.stages = std::min<int>(kNMaxStages, kNStageSpace / (kWeights<kMode> + p.columns * kFfnK * 2));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = (unsigned)(tiles * cluster);
+    cfg.blockDim = kNThreads;
+    cfg.dynamicSmemBytes = kNSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = follows ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, narrow_kernel<kMode>, p);
+  }
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail_ffn(LTXATTN_ERR_CUDA, "%s: %s", call, cudaGetErrorString(e));
+  }
+  return LTXATTN_OK;
+}
+
+}  // namespace
+
+int launch_narrow(NarrowMode mode, NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
+  p.tiles = (int)div_up(p.features, kNRows);
+  p.err = device_error_word();
+  if (!p.err) return fail_ffn(LTXATTN_ERR_CUDA, "no device error word");
+  switch (mode) {
+    case kNarrowProduct: return launch<kNarrowProduct>(p, follows, call, st);
+    case kNarrowStore: return launch<kNarrowStore>(p, follows, call, st);
+    case kNarrowSlopes: return launch<kNarrowSlopes>(p, follows, call, st);
+    default: return launch<kNarrowStoreMN>(p, follows, call, st);
+  }
+}
+
+}  // namespace ltx

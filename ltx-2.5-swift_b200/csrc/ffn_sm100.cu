@@ -34,9 +34,7 @@
 #include <cstdio>
 #include <mutex>
 
-#include "../../include/ltxattn.h"
-#include "ltxattn_internal.h"
-#include "sm100.cuh"
+#include "ffn_common.cuh"
 
 namespace ltx {
 
@@ -46,7 +44,7 @@ namespace {
 
 constexpr int kGM = 128;       // rows of a tile (UMMA M)
 constexpr int kGN = 256;       // accumulator columns of a tile (UMMA N)
-constexpr int kGK = 64;        // K per stage: one 128-byte swizzle row of bf16
+constexpr int kGK = kFfnK;
 constexpr int kGStages = 4;
 constexpr int kGThreads = 384;  // 4 control warps, 8 epilogue warps
 constexpr uint32_t kGA = kGM * kGK * 2;
@@ -81,44 +79,6 @@ struct GemmParams {
   int64_t gate_stride, up_stride, dgate_stride, dup_stride;
   int* err;
 };
-
-// ---------------------------------------------------------------------------
-// activations (fp32)
-
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
-
-// act(g), and with kSlope its derivative too.
-template <bool kSlope>
-__device__ __forceinline__ float activate(int kind, float g, float& slope) {
-  if (kind == LTXATTN_SILU) {
-    const float s = sigmoid(g);
-    if (kSlope) slope = s * fmaf(g, 1.0f - s, 1.0f);
-    return g * s;
-  }
-  if (kind == LTXATTN_GELU_TANH) {
-    // (1 + tanh z) / 2 = sigmoid(2 z)
-    constexpr float c2 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
-    const float g2 = g * g;
-    const float s = sigmoid(c2 * g * fmaf(0.044715f, g2, 1.0f));
-    if (kSlope) {
-      const float t = g * s * (1.0f - s);  // 0 far out, where g2 may be infinite
-      slope = t == 0.0f ? s : fmaf(t, c2 * fmaf(0.134145f, g2, 1.0f), s);
-    }
-    return g * s;
-  }
-  const float s = 0.5f * erfcf(-0.70710678118654752f * g);
-  if (kSlope) slope = fmaf(g, 0.3989422804014327f * __expf(-0.5f * g * g), s);
-  return g * s;
-}
-
-__device__ __forceinline__ float lo_f(uint32_t v) { return __uint_as_float(v << 16); }
-__device__ __forceinline__ float hi_f(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
-
-// 8 consecutive bf16 of a row (16-byte aligned).
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                                            pack_bf16x2(v[6], v[7]));
-}
 
 // ---------------------------------------------------------------------------
 
@@ -302,20 +262,11 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[8 * q + e]);
             if (kEpilogue == kSlopes) {
-              const uint4 g4 = *reinterpret_cast<const uint4*>(p.gate + row * p.gate_stride + col + 8 * q);
-              const uint4 u4 = *reinterpret_cast<const uint4*>(p.up + row * p.up_stride + col + 8 * q);
-              const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
-              float dgv[8], duv[8];
+              float gv[8], uv[8], dgv[8], duv[8];
+              load8(p.gate + row * p.gate_stride + col + 8 * q, gv);
+              load8(p.up + row * p.up_stride + col + 8 * q, uv);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float gv = (e & 1) ? hi_f(gw[e / 2]) : lo_f(gw[e / 2]);
-                const float uv = (e & 1) ? hi_f(uw[e / 2]) : lo_f(uw[e / 2]);
-                float slope;
-                const float a = activate<true>(p.activation, gv, slope);
-                dgv[e] = v[e] * uv * slope;
-                duv[e] = v[e] * a;
-                v[e] = a * uv;
-              }
+              for (int e = 0; e < 8; ++e) slopes(p.activation, gv[e], uv[e], v[e], dgv[e], duv[e], v[e]);
               store8(p.dgate + row * p.dgate_stride + col + 8 * q, dgv);
               store8(p.dup + row * p.dup_stride + col + 8 * q, duv);
               if (g.out == nullptr) continue;  // h is wanted for dw_down alone
@@ -359,6 +310,8 @@ EncodeTiledFn encoder() {
   return fn;
 }
 
+}  // namespace
+
 int fail_ffn(int status, const char* fmt, ...) {
   char buf[512];
   va_list ap;
@@ -368,9 +321,8 @@ int fail_ffn(int status, const char* fmt, ...) {
   return set_error_message(status, buf);
 }
 
-// bf16 [rows, cols], `stride` elements between rows; boxes of 64 columns (one swizzle row) and box_rows rows.
-int map_2d(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t stride, int box_rows,
-           const char* name) {
+int ffn_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t stride, int box_rows,
+            const char* name) {
   EncodeTiledFn enc = encoder();
   if (!enc) return fail_ffn(LTXATTN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
@@ -384,6 +336,8 @@ int map_2d(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t 
     return fail_ffn(LTXATTN_ERR_ALIGN, "%s: cuTensorMapEncodeTiled rejected the view (CUresult %d)", name, (int)r);
   return LTXATTN_OK;
 }
+
+namespace {
 
 // A bf16 matrix argument.
 struct Mat {
@@ -440,8 +394,6 @@ cudaError_t prepare_kernel(K kernel, int slot, int* sms) {
   return cudaSuccess;
 }
 
-int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 template <bool kAMN, bool kBMN, int kEpilogue>
 int launch_gemm(GemmParams& p, int slot, const char* call, cudaStream_t st) {
   const int width = kEpilogue == kProduct ? kGN / 2 : kGN;
@@ -470,6 +422,9 @@ int launch_gemm(GemmParams& p, int slot, const char* call, cudaStream_t st) {
   }
   return LTXATTN_OK;
 }
+
+// Up to this many tokens the products run feature by feature (ffn_narrow_sm100.cu).
+constexpr int kNarrowTokens = 128;
 
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
@@ -516,13 +471,45 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   __nv_bfloat16* h = static_cast<__nv_bfloat16*>(a->workspace);
 
+  if (a->m <= kNarrowTokens) {
+    NarrowParams p{};
+    p.tokens = a->m;
+    p.columns = narrow_columns(a->m);
+    p.features = a->inner;
+    p.kb = p.kb_first = (int)div_up(a->hidden, kFfnK);
+    p.activation = a->activation;
+    p.out = h;
+    p.out_stride = a->inner;
+    p.gate = static_cast<__nv_bfloat16*>(a->gate);
+    p.up = static_cast<__nv_bfloat16*>(a->up);
+    p.gate_stride = a->gate_stride;
+    p.up_stride = a->up_stride;
+    const int box = narrow_box(kNarrowProduct);
+    if (int rc = ffn_map(&p.a[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, box, "w_gate")) return rc;
+    if (int rc = ffn_map(&p.a[1], a->w_up, a->inner, a->hidden, a->w_up_stride, box, "w_up")) return rc;
+    if (int rc = ffn_map(&p.b[0], a->x, a->m, a->hidden, a->x_stride, p.columns, "x")) return rc;
+    if (int rc = launch_narrow(kNarrowProduct, p, false, call, st)) return rc;
+
+    NarrowParams d{};
+    d.tokens = a->m;
+    d.columns = p.columns;
+    d.features = a->out_dim;
+    d.kb = d.kb_first = (int)div_up(a->inner, kFfnK);
+    d.out = static_cast<__nv_bfloat16*>(a->out);
+    d.out_stride = a->out_stride;
+    if (int rc = ffn_map(&d.a[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, narrow_box(kNarrowStore), "w_down"))
+      return rc;
+    if (int rc = ffn_map(&d.b[0], h, a->m, a->inner, a->inner, d.columns, "workspace")) return rc;
+    return launch_narrow(kNarrowStore, d, true, call, st);
+  }
+
   GemmParams p{};
   p.count = 1;
   p.activation = a->activation;
   Gemm& g = p.g[0];
-  if (int rc = map_2d(&g.a[0], a->x, a->m, a->hidden, a->x_stride, kGM, "x")) return rc;
-  if (int rc = map_2d(&g.b[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, kGN / 2, "w_gate")) return rc;
-  if (int rc = map_2d(&g.b[1], a->w_up, a->inner, a->hidden, a->w_up_stride, kGN / 2, "w_up")) return rc;
+  if (int rc = ffn_map(&g.a[0], a->x, a->m, a->hidden, a->x_stride, kGM, "x")) return rc;
+  if (int rc = ffn_map(&g.b[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, kGN / 2, "w_gate")) return rc;
+  if (int rc = ffn_map(&g.b[1], a->w_up, a->inner, a->hidden, a->w_up_stride, kGN / 2, "w_up")) return rc;
   g.M = a->m;
   g.N = a->inner;
   g.kb = g.kb_first = (int)div_up(a->hidden, kGK);
@@ -537,8 +524,8 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
   GemmParams d{};
   d.count = 1;
   Gemm& o = d.g[0];
-  if (int rc = map_2d(&o.a[0], h, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
-  if (int rc = map_2d(&o.b[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, kGN, "w_down")) return rc;
+  if (int rc = ffn_map(&o.a[0], h, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
+  if (int rc = ffn_map(&o.b[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, kGN, "w_down")) return rc;
   o.M = a->m;
   o.N = a->out_dim;
   o.kb = o.kb_first = (int)div_up(a->inner, kGK);
@@ -600,20 +587,59 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
   __nv_bfloat16* dup = reinterpret_cast<__nv_bfloat16*>(ws + plane);
   __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(ws + 2 * plane);
 
-  {  // dh = dout w_down, and what follows from it element by element
+  __nv_bfloat16* gate = static_cast<__nv_bfloat16*>(const_cast<void*>(a->gate));
+  __nv_bfloat16* up = static_cast<__nv_bfloat16*>(const_cast<void*>(a->up));
+  const bool narrow = a->m <= kNarrowTokens;
+  // dh = dout w_down, and what follows from it element by element; then dx
+  if (narrow) {
+    NarrowParams p{};
+    p.tokens = a->m;
+    p.columns = narrow_columns(a->m);
+    p.features = a->inner;
+    p.kb = p.kb_first = (int)div_up(a->out_dim, kFfnK);
+    p.activation = a->activation;
+    p.out = a->dw_down != nullptr ? h : nullptr;
+    p.out_stride = p.dgate_stride = p.dup_stride = a->inner;
+    p.gate = gate;
+    p.up = up;
+    p.gate_stride = a->gate_stride;
+    p.up_stride = a->up_stride;
+    p.dgate = dgate;
+    p.dup = dup;
+    if (int rc = ffn_map(&p.a[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, narrow_box(kNarrowSlopes), "w_down"))
+      return rc;
+    if (int rc = ffn_map(&p.b[0], a->dout, a->m, a->out_dim, a->dout_stride, p.columns, "dout")) return rc;
+    if (int rc = launch_narrow(kNarrowSlopes, p, false, call, st)) return rc;
+    if (a->dx != nullptr) {
+      NarrowParams d{};
+      d.tokens = a->m;
+      d.columns = p.columns;
+      d.features = a->hidden;
+      d.kb_first = (int)div_up(a->inner, kFfnK);
+      d.kb = 2 * d.kb_first;
+      d.out = static_cast<__nv_bfloat16*>(a->dx);
+      d.out_stride = a->dx_stride;
+      const int box = narrow_box(kNarrowStoreMN);
+      if (int rc = ffn_map(&d.a[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, box, "w_gate")) return rc;
+      if (int rc = ffn_map(&d.a[1], a->w_up, a->inner, a->hidden, a->w_up_stride, box, "w_up")) return rc;
+      if (int rc = ffn_map(&d.b[0], dgate, a->m, a->inner, a->inner, d.columns, "workspace")) return rc;
+      if (int rc = ffn_map(&d.b[1], dup, a->m, a->inner, a->inner, d.columns, "workspace")) return rc;
+      if (int rc = launch_narrow(kNarrowStoreMN, d, true, call, st)) return rc;
+    }
+  } else {
     GemmParams p{};
     p.count = 1;
     p.activation = a->activation;
     Gemm& g = p.g[0];
-    if (int rc = map_2d(&g.a[0], a->dout, a->m, a->out_dim, a->dout_stride, kGM, "dout")) return rc;
-    if (int rc = map_2d(&g.b[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, kGK, "w_down")) return rc;
+    if (int rc = ffn_map(&g.a[0], a->dout, a->m, a->out_dim, a->dout_stride, kGM, "dout")) return rc;
+    if (int rc = ffn_map(&g.b[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, kGK, "w_down")) return rc;
     g.M = a->m;
     g.N = a->inner;
     g.kb = g.kb_first = (int)div_up(a->out_dim, kGK);
     g.out = a->dw_down != nullptr ? h : nullptr;
     g.out_stride = a->inner;
-    p.gate = static_cast<__nv_bfloat16*>(const_cast<void*>(a->gate));
-    p.up = static_cast<__nv_bfloat16*>(const_cast<void*>(a->up));
+    p.gate = gate;
+    p.up = up;
     p.gate_stride = a->gate_stride;
     p.up_stride = a->up_stride;
     p.dgate = dgate;
@@ -621,14 +647,14 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     p.dgate_stride = p.dup_stride = a->inner;
     if (int rc = launch_gemm<false, true, kSlopes>(p, 2, call, st)) return rc;
   }
-  if (a->dx != nullptr) {
+  if (!narrow && a->dx != nullptr) {
     GemmParams p{};
     p.count = 1;
     Gemm& g = p.g[0];
-    if (int rc = map_2d(&g.a[0], dgate, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
-    if (int rc = map_2d(&g.a[1], dup, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
-    if (int rc = map_2d(&g.b[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, kGK, "w_gate")) return rc;
-    if (int rc = map_2d(&g.b[1], a->w_up, a->inner, a->hidden, a->w_up_stride, kGK, "w_up")) return rc;
+    if (int rc = ffn_map(&g.a[0], dgate, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
+    if (int rc = ffn_map(&g.a[1], dup, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
+    if (int rc = ffn_map(&g.b[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, kGK, "w_gate")) return rc;
+    if (int rc = ffn_map(&g.b[1], a->w_up, a->inner, a->hidden, a->w_up_stride, kGK, "w_up")) return rc;
     g.M = a->m;
     g.N = a->hidden;
     g.kb_first = (int)div_up(a->inner, kGK);
@@ -642,8 +668,8 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
                     int64_t out_stride, const char* an, const char* bn) {
     if (out == nullptr) return (int)LTXATTN_OK;
     Gemm& g = p.g[p.count++];
-    if (int rc = map_2d(&g.a[0], at, a->m, rows, at_stride, kGK, an)) return rc;
-    if (int rc = map_2d(&g.b[0], b, a->m, cols, b_stride, kGK, bn)) return rc;
+    if (int rc = ffn_map(&g.a[0], at, a->m, rows, at_stride, kGK, an)) return rc;
+    if (int rc = ffn_map(&g.b[0], b, a->m, cols, b_stride, kGK, bn)) return rc;
     g.M = rows;
     g.N = cols;
     g.kb = g.kb_first = (int)div_up(a->m, kGK);
