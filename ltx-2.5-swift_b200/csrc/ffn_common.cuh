@@ -14,7 +14,8 @@ namespace ltx {
 // ---------------------------------------------------------------------------
 // activations (fp32)
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
+// The fast division is off by 2 units of 2^-24; 1 + e^-x is at most infinite, and then it gives 0.
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
 // act(g), and with kSlope its derivative too.
 template <bool kSlope>
@@ -91,6 +92,7 @@ struct NarrowParams {
   int columns;           // tokens of a tile: a multiple of 16, the box of b
   int tiles;             // feature tiles
   int stages;
+  int follows;           // the kernel before it in the stream belongs to the same call
   int activation;
   __nv_bfloat16* out;    // [tokens, features]
   int64_t out_stride;
@@ -112,7 +114,7 @@ constexpr int kNarrowColumns = 128;  // tokens of a tile at most
 inline int narrow_columns(int tokens) { return tokens >= kNarrowColumns ? kNarrowColumns : (int)div_up(tokens, 16) * 16; }
 // Rows of the boxes of a[]: 128 features K-major, 64 of K MN-major.
 inline int narrow_box(NarrowMode mode) { return mode == kNarrowProduct || mode == kNarrowStore ? 128 : kFfnK; }
-// `follows`: the kernel reads what the one before it in the stream wrote, and may start while that one ends.
+// `follows`: the kernel before it in the stream belongs to the same call and does not write the weights.
 int launch_narrow(NarrowMode mode, NarrowParams& p, bool follows, const char* call, cudaStream_t st);
 
 }  // namespace ltx

@@ -28,18 +28,19 @@ namespace {
 
 constexpr int kNThreads = 384;  // 4 control warps, 8 epilogue warps
 constexpr int kNRows = 128;     // features of a tile (UMMA M)
-constexpr int kNMaxStages = 12;
+constexpr int kNMaxStages = 6;
 constexpr int kNMaxCluster = 8;
 constexpr uint32_t kNATile = kNRows * kFfnK * 2;
 constexpr uint32_t kNChunk = 64 * kFfnK * 2;  // MN-major: 64 features x 64 rows of K
-constexpr uint32_t kNStageSpace = 216 * 1024;
+constexpr uint32_t kNStageSpace = 108 * 1024;  // two CTAs to an SM
 // full, empty per stage, acc_full
 constexpr uint32_t kNOffBar = kNStageSpace;
 constexpr uint32_t kNOffCtl = kNOffBar + (2 * kNMaxStages + 1) * 8;
 constexpr uint32_t kNSmem = kNOffCtl + 16 + 1024;  // + alignment slack
-static_assert(kNSmem <= kMaxDynamicSmem, "shared memory of a CTA");
-// a tile's partial sums, [accumulator column][128 features] fp32, take the stages' place
-static_assert(2 * kNarrowColumns * kNRows * 4 <= kNStageSpace, "partial sums");
+static_assert(2 * (kNSmem + 1024) <= 228 * 1024, "two CTAs to an SM");
+// Partial sums, [accumulator column][128 features] fp32, take the stages' place: of so many tokens at a time.
+template <NarrowMode kMode>
+constexpr int kExchange = kNStageSpace / (kNRows * 4) / (kMode == kNarrowProduct ? 2 : 1) / 8 * 8;
 
 // bytes of the weights in a stage
 template <NarrowMode kMode>
@@ -76,19 +77,35 @@ __device__ __forceinline__ float4 peer_load4(uint32_t local, uint32_t rank) {
   return v;
 }
 
-// The sum over the cluster's parts of 8 features (from `feature`) of one accumulator column.
-__device__ __forceinline__ void sum8(uint32_t partial, int column, int feature, uint32_t ranks, float (&v)[8]) {
-  const uint32_t at = partial + (column * kNRows + feature) * 4;
-  for (uint32_t r = 0; r < ranks; ++r) {
-    const float4 a = peer_load4(at, r), b = peer_load4(at + 16, r);
-    const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+// The cluster's parts of 4 features (from `feature`) of one accumulator column.
+struct Parts {
+  float4 part[kNMaxCluster];
+
+  // all on their way at once: a read of another CTA's shared memory takes a few hundred ns
+  __device__ __forceinline__ void load(uint32_t partial, int column, int feature, uint32_t ranks) {
+    const uint32_t at = partial + (column * kNRows + feature) * 4;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = r == 0 ? w[e] : v[e] + w[e];
+    for (uint32_t r = 0; r < kNMaxCluster; ++r)
+      if (r < ranks) part[r] = peer_load4(at, r);
   }
+  __device__ __forceinline__ void sum(uint32_t ranks, float (&v)[4]) const {
+    v[0] = part[0].x, v[1] = part[0].y, v[2] = part[0].z, v[3] = part[0].w;
+#pragma unroll
+    for (uint32_t r = 1; r < kNMaxCluster; ++r)
+      if (r < ranks) v[0] += part[r].x, v[1] += part[r].y, v[2] += part[r].z, v[3] += part[r].w;
+  }
+};
+
+// 4 consecutive bf16 of a row (8-byte aligned).
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+__device__ __forceinline__ void unpack4(const uint2& w, float (&v)[4]) {
+  v[0] = lo_f(w.x), v[1] = hi_f(w.x), v[2] = lo_f(w.y), v[3] = hi_f(w.y);
 }
 
 template <NarrowMode kMode>
-__global__ void __launch_bounds__(kNThreads, 1) narrow_kernel(const __grid_constant__ NarrowParams p) {
+__global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_constant__ NarrowParams p) {
   constexpr bool kDual = kMode == kNarrowProduct;
   constexpr bool kAMN = kMode == kNarrowSlopes || kMode == kNarrowStoreMN;
   extern __shared__ uint8_t smem_raw[];
@@ -107,9 +124,7 @@ __global__ void __launch_bounds__(kNThreads, 1) narrow_kernel(const __grid_const
   const int kb_n = kb1 - kb0;  // >= 1: there are no more ranks than K slices
   const uint32_t stage_bytes = kWeights<kMode> + p.columns * kFfnK * 2;
   const int stages = p.stages;
-  const int acc_columns = kDual ? 2 * p.columns : p.columns;
-  uint32_t tmem_columns = 32;
-  while ((int)tmem_columns < acc_columns) tmem_columns *= 2;
+  constexpr uint32_t tmem_columns = (kDual ? 2 : 1) * kNarrowColumns;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < stages; ++i) {
@@ -153,9 +168,12 @@ __global__ void __launch_bounds__(kNThreads, 1) narrow_kernel(const __grid_const
       const int k0 = (part ? kb - p.kb_first : kb) * kFfnK;
       tma_load_2d(&p.b[part], full + st, sm + st * stage_bytes + kWeights<kMode>, k0, t0);
     };
+    // The second product of a call need not wait for the first to load its weights, only to load its tokens.
+    // The first one waits for whatever was before it in the stream, which may have written anything.
     const int first = min(stages, kb_n);
+    if (!p.follows) grid_dep_wait();
     for (int i = 0; i < first; ++i) weights(i);
-    grid_dep_wait();  // what the tokens' operand is read from is written by the kernel before
+    if (p.follows) grid_dep_wait();
     for (int i = 0; i < first; ++i) tokens(i);
     int i = first;
     for (; i < kb_n; ++i) {
@@ -190,66 +208,81 @@ __global__ void __launch_bounds__(kNThreads, 1) narrow_kernel(const __grid_const
   }
   __syncwarp();
 
-  // this CTA's partial sums, where the stages were: acc_full comes after the last MMA's reads, and every
-  // copy has landed before an MMA that read it
+  // the partial sums go where the stages were: acc_full comes after the last MMA's reads, and every copy has
+  // landed before an MMA that read it
   const uint32_t partial = smem_u32(sm);
-  if (warp >= 4) {
-    const bool have = warp_wait(acc_full, 0, abort_flag, p.err, 67);
-    tc_fence_after();
-    const int quadrant = warp & 3;
-    float* row = reinterpret_cast<float*>(sm) + quadrant * 32 + lane;
-    if (have) {
-      for (int c = ((warp - 4) >> 2) * 16; c < acc_columns; c += 32) {
-        __syncwarp();
-        uint32_t r[16];
-        tmem_ld16(tmem + (static_cast<uint32_t>(quadrant * 32) << 16) + c, r);
-        tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 16; ++e) row[(c + e) * kNRows] = __uint_as_float(r[e]);
-      }
-    }
-    tc_fence_before();
-  }
-  __syncthreads();
-  cluster_barrier();
-
-  // the cluster's CTAs share the tile's tokens; a thread finishes 8 features of one
   const int n_tokens = min(p.columns, p.tokens - t0);
-  const int first = (int)(n_tokens * rank / ranks), last = (int)(n_tokens * (rank + 1) / ranks);
-  if (warp >= 4 && *abort_flag == 0) {
-    const int i = threadIdx.x - 128;
-    const int col = f0 + (i % 16) * 8;
-    for (int t = first + i / 16; t < last; t += 16) {
-      if (col >= p.features) break;
-      const int64_t token = t0 + t;
-      float v[8];
-      sum8(partial, t, (i % 16) * 8, ranks, v);
-      if (kDual) {
-        float u[8];
-        sum8(partial, p.columns + t, (i % 16) * 8, ranks, u);
-        if (p.gate != nullptr) {
-          store8(p.gate + token * p.gate_stride + col, v);
-          store8(p.up + token * p.up_stride + col, u);
-        }
-        float unused;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = activate<false>(p.activation, v[e], unused) * u[e];
-      }
-      if (kMode == kNarrowSlopes) {
-        float g[8], u[8], dg[8], du[8];
-        load8(p.gate + token * p.gate_stride + col, g);
-        load8(p.up + token * p.up_stride + col, u);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) slopes(p.activation, g[e], u[e], v[e], dg[e], du[e], v[e]);
-        store8(p.dgate + token * p.dgate_stride + col, dg);
-        store8(p.dup + token * p.dup_stride + col, du);
-        if (p.out == nullptr) continue;  // h is wanted for dw_down alone
-      }
-      store8(p.out + token * p.out_stride + col, v);
-    }
+  bool have = false;
+  if (warp >= 4) {
+    have = warp_wait(acc_full, 0, abort_flag, p.err, 67);
+    tc_fence_after();
   }
+  for (int c0 = 0; c0 < n_tokens; c0 += kExchange<kMode>) {
+    const int n = min(kExchange<kMode>, n_tokens - c0);
+    if (have) {
+      const int quadrant = warp & 3;
+      float* row = reinterpret_cast<float*>(sm) + quadrant * 32 + lane;
+      const uint32_t at = tmem + (static_cast<uint32_t>(quadrant * 32) << 16) + c0;
+      for (int c = ((warp - 4) >> 2) * 16; c < n; c += 32) {
+#pragma unroll
+        for (int part = 0; part < (kDual ? 2 : 1); ++part) {
+          __syncwarp();
+          uint32_t r[16];
+          tmem_ld16(at + part * p.columns + c, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (c + e < kExchange<kMode>) row[(part * kExchange<kMode> + c + e) * kNRows] = __uint_as_float(r[e]);
+        }
+      }
+    }
+    __syncthreads();
+    cluster_barrier();
+    // the cluster's CTAs share the tokens; a thread finishes 4 features of one
+    const int first = (int)(n * rank / ranks), last = (int)(n * (rank + 1) / ranks);
+    const int feature = lane * 4, col = f0 + feature;
+    if (*abort_flag == 0 && col < p.features) {
+      for (int t = first + warp; t < last; t += kNThreads / 32) {
+        const int64_t token = t0 + c0 + t;
+        uint2 gate, up;
+        if (kMode == kNarrowSlopes) {
+          gate = *reinterpret_cast<const uint2*>(p.gate + token * p.gate_stride + col);
+          up = *reinterpret_cast<const uint2*>(p.up + token * p.up_stride + col);
+        }
+        Parts a, b;
+        a.load(partial, t, feature, ranks);
+        if (kDual) b.load(partial, kExchange<kMode> + t, feature, ranks);
+        float v[4];
+        a.sum(ranks, v);
+        if (kDual) {
+          float u[4];
+          b.sum(ranks, u);
+          if (p.gate != nullptr) {
+            store4(p.gate + token * p.gate_stride + col, v);
+            store4(p.up + token * p.up_stride + col, u);
+          }
+          float unused;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = activate<false>(p.activation, v[e], unused) * u[e];
+        }
+        if (kMode == kNarrowSlopes) {
+          float g[4], u[4], dg[4], du[4];
+          unpack4(gate, g);
+          unpack4(up, u);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) slopes(p.activation, g[e], u[e], v[e], dg[e], du[e], v[e]);
+          store4(p.dgate + token * p.dgate_stride + col, dg);
+          store4(p.dup + token * p.dup_stride + col, du);
+          if (p.out == nullptr) continue;  // h is wanted for dw_down alone
+        }
+        store4(p.out + token * p.out_stride + col, v);
+      }
+    }
+    __syncthreads();
+    cluster_barrier();  // no CTA leaves, or writes the next tokens' sums, while another reads these
+  }
+  if (warp >= 4) tc_fence_before();
   __syncthreads();
-  cluster_barrier();  // no CTA leaves while another reads its partial sums
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, tmem_columns);
@@ -275,6 +308,9 @@ cudaError_t prepare(Occupancy* out) {
   Occupancy& o = g_occupancy[dev][kMode];
   if (!o.ready) {
     e = cudaFuncSetAttribute(narrow_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(narrow_kernel<kMode>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                               cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
     for (int s = 1; s <= kNMaxCluster; ++s) {
       cudaLaunchConfig_t cfg = {};
@@ -296,21 +332,17 @@ cudaError_t prepare(Occupancy* out) {
   return cudaSuccess;
 }
 
-// CTAs that share a tile: the size that ends first, counting rounds of clusters
-// over the SMs, K slices of a CTA, and what a round costs besides (about four
-// slices: filling the pipeline, the exchange, the epilogue).
+// CTAs that share a tile: as many as fit the GPU at once, two to an SM (the
+// occupancy query counts one, as for every kernel that allocates TMEM; two run),
+// and leave each CTA four K slices.  More CTAs keep more loads in flight -- the
+// bandwidth needs about 13 MB of them -- but from some 250 on the exchange costs
+// more than that gives.  For 19 tokens at 2048 x 8192, 2, 3 and 4 CTAs to a tile
+// of the first product took 35.3, 34.0 and 33.0 us for both; for one token at
+// 4096 x 16384, 4, 5, 6 and 8 of the second 81.9, 76.8, 75.0 and 77.6.
 int choose_cluster(const Occupancy& o, int64_t tiles, int kb) {
-  int best = 1;
-  int64_t best_cost = -1;
-  for (int s = 1; s <= std::min(kNMaxCluster, kb); ++s) {
-    if (o.clusters[s] < 1) continue;
-    const int64_t cost = div_up(tiles, o.clusters[s]) * (div_up(kb, s) + 4);
-    if (best_cost < 0 || cost < best_cost) {
-      best = s;
-      best_cost = cost;
-    }
-  }
-  return best;
+  for (int s = std::min(kNMaxCluster, kb / 4); s > 1; --s)
+    if (tiles <= 2 * o.clusters[s] && tiles * s <= 256) return s;
+  return 1;
 }
 
 template <NarrowMode kMode>
@@ -334,7 +366,8 @@ int launch(NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = follows ? 2 : 1;
+    cfg.numAttrs = 2;
+    p.follows = follows;
     e = cudaLaunchKernelEx(&cfg, narrow_kernel<kMode>, p);
   }
   if (e != cudaSuccess) {

@@ -49,23 +49,37 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str = "
     return torch.tensor(list(out), dtype=torch.float64).to(device), magnitude.value
 
 
-def _heads(name: str, t: torch.Tensor, shape: tuple, dtype, device: int) -> _lib.Tensor:
-    """The view of a [B, heads, tokens, D] tensor on that device."""
+def _on_device(name: str, t, device: int):
+    """Refuses what is no CUDA tensor, or one on another device than q."""
     _check_cuda(name, t)
+    if t.get_device() != device:
+        raise Failure("arg", f"{name} is on {t.device}, q on cuda:{device}", _lib.ERR_ARG)
+
+
+def _heads(name: str, t: torch.Tensor, shape: tuple, dtype, device: int) -> _lib.Tensor:
+    """The view of a [B, heads, tokens, D] tensor."""
+    _on_device(name, t, device)
     if t.shape != shape:
         raise Failure.shape(name, t.shape, str(list(shape)))
     if t.dtype != dtype:
         raise Failure("dtype", f"{name} is {t.dtype}, q is {dtype}", _lib.ERR_DTYPE)
-    _same_device(name, t, device)
     sb, sh, st, sd = t.stride()
     if sd != 1:
         raise Failure("align", f"{name} must have a unit stride in its last dim", _lib.ERR_ALIGN)
     return _lib.Tensor(t.data_ptr(), sb, sh, st)
 
 
-def _same_device(name: str, t: torch.Tensor, device: int):
-    if t.get_device() != device:
-        raise Failure("arg", f"{name} is on {t.device}, q on cuda:{device}", _lib.ERR_ARG)
+def _new_like(t: torch.Tensor):
+    """An output in the layout of its input, and its view."""
+    out = torch.empty_like(t)
+    sb, sh, st, sd = out.stride()
+    if sd != 1:
+        out = t.new_empty(t.shape)
+        sb, sh, st, sd = out.stride()
+    return out, _lib.Tensor(out.data_ptr(), sb, sh, st)
+
+
+_NO_HEADS = _lib.Tensor()
 
 
 def _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k, stream, inverse):
@@ -76,45 +90,43 @@ def _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k
     B, H, T, D = shape
     if layout not in LAYOUTS:
         raise Failure("arg", f"layout {layout!r} is neither 'half' nor 'interleaved'", _lib.ERR_ARG)
-    _check_cuda("frequencies", frequencies)
-    _same_device("frequencies", frequencies, device)
+    _on_device("frequencies", frequencies, device)
     if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
         raise Failure.shape("frequencies", frequencies.shape, "[rotaryDim / 2] float64, contiguous")
-    a = _lib.RotaryEmbedArgs(_dtype_code(q), B, T, H, 0, D, 2 * frequencies.shape[0], LAYOUTS[layout],
-                             1 if inverse else 0, magnitude)
-    a.frequencies, a.offset = frequencies.data_ptr(), offset
-    a.q = _heads("q", q, shape, dtype, device)
+    vq = _heads("q", q, shape, dtype, device)
+    kv_heads, vk, v_out_k = 0, _NO_HEADS, _NO_HEADS
     if k is not None:
-        if k.dim() != 4:
-            raise Failure.shape("k", k.shape, f"[{B}, kvHeads, {T}, {D}]")
-        k_shape = (B, k.shape[1], T, D)
-        a.kv_heads, a.k = k_shape[1], _heads("k", k, k_shape, dtype, device)
+        _on_device("k", k, device)
+        kv_heads = k.shape[1] if k.dim() == 4 else 0
+        k_shape = (B, kv_heads, T, D)
+        vk = _heads("k", k, k_shape, dtype, device)
     elif out_k is not None:
         raise Failure("arg", "out_k without k", _lib.ERR_ARG)
+    at, bits, at_sb, at_st = None, 0, 0, 0
     if positions is not None:
-        _check_cuda("positions", positions)
-        _same_device("positions", positions, device)
-        if positions.dtype == torch.int64:
-            a.position_bits = 64
-        elif positions.dtype == torch.int32:
-            a.position_bits = 32
-        else:
+        _on_device("positions", positions, device)
+        if positions.dtype != torch.int64 and positions.dtype != torch.int32:
             raise Failure("dtype", f"positions are {positions.dtype}, expected int64 or int32", _lib.ERR_DTYPE)
-        p_shape = tuple(positions.shape)
+        p_shape = positions.shape
         if p_shape != (B, T) and p_shape != (T,) and p_shape != (1, T):
             raise Failure.shape("positions", p_shape, f"[{T}] or [1|{B}, {T}]")
         strides = positions.stride()
-        a.positions, a.position_stride_t = positions.data_ptr(), strides[-1]
+        at, bits, at_st = positions.data_ptr(), 8 * positions.element_size(), strides[-1]
         if len(p_shape) == 2 and p_shape[0] > 1:
-            a.position_stride_b = strides[0]
+            at_sb = strides[0]
     with _on(device, stream) as st:
         if out_q is None:
-            out_q = torch.empty_like(q)
-        a.q_out = _heads("out_q", out_q, shape, dtype, device)
+            out_q, v_out_q = _new_like(q)
+        else:
+            v_out_q = _heads("out_q", out_q, shape, dtype, device)
         if k is not None:
             if out_k is None:
-                out_k = torch.empty_like(k)
-            a.k_out = _heads("out_k", out_k, k_shape, dtype, device)
+                out_k, v_out_k = _new_like(k)
+            else:
+                v_out_k = _heads("out_k", out_k, k_shape, dtype, device)
+        a = _lib.RotaryEmbedArgs(_dtype_code(q), B, T, H, kv_heads, D, 2 * frequencies.shape[0], LAYOUTS[layout],
+                                 1 if inverse else 0, magnitude, vq, v_out_q, vk, v_out_k, frequencies.data_ptr(), at,
+                                 bits, at_sb, at_st, offset)
         rc = _lib.load().ltxattn_rotary_embed(ctypes.byref(a), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
