@@ -26,7 +26,7 @@ namespace ltx {
 
 namespace {
 
-constexpr int kNThreads = 384;  // 4 control warps, 8 epilogue warps
+constexpr int kNThreads = 256;  // 8 warps: a producer, an MMA issuer, and then all for the epilogue
 constexpr int kNRows = 128;     // features of a tile (UMMA M)
 constexpr int kNMaxStages = 6;
 constexpr int kNMaxCluster = 8;
@@ -65,11 +65,19 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// 4 floats at the address that `local` has in this CTA, of the CTA with that rank.
-__device__ __forceinline__ float4 peer_load4(uint32_t local, uint32_t rank) {
+// 4 floats at the address that `local` has in this CTA, of the CTA with that rank (of this one: without the
+// way through the cluster's network, which gives some 10 bytes a cycle to an SM).
+__device__ __forceinline__ float4 peer_load4(uint32_t local, uint32_t rank, uint32_t own) {
+  float4 v;
+  if (rank == own) {
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(local)
+                 : "memory");
+    return v;
+  }
   uint32_t at;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
-  float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                : "r"(at)
@@ -82,11 +90,11 @@ struct Parts {
   float4 part[kNMaxCluster];
 
   // all on their way at once: a read of another CTA's shared memory takes a few hundred ns
-  __device__ __forceinline__ void load(uint32_t partial, int column, int feature, uint32_t ranks) {
+  __device__ __forceinline__ void load(uint32_t partial, int column, int feature, uint32_t ranks, uint32_t own) {
     const uint32_t at = partial + (column * kNRows + feature) * 4;
 #pragma unroll
     for (uint32_t r = 0; r < kNMaxCluster; ++r)
-      if (r < ranks) part[r] = peer_load4(at, r);
+      if (r < ranks) part[r] = peer_load4(at, r, own);
   }
   __device__ __forceinline__ void sum(uint32_t ranks, float (&v)[4]) const {
     v[0] = part[0].x, v[1] = part[0].y, v[2] = part[0].z, v[3] = part[0].w;
@@ -212,28 +220,27 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
   // landed before an MMA that read it
   const uint32_t partial = smem_u32(sm);
   const int n_tokens = min(p.columns, p.tokens - t0);
-  bool have = false;
-  if (warp >= 4) {
-    have = warp_wait(acc_full, 0, abort_flag, p.err, 67);
-    tc_fence_after();
-  }
-  for (int c0 = 0; c0 < n_tokens; c0 += kExchange<kMode>) {
-    const int n = min(kExchange<kMode>, n_tokens - c0);
+  const bool have = warp_wait(acc_full, 0, abort_flag, p.err, 67);
+  tc_fence_after();
+  // TMEM is read 16 columns at a time: pieces start at multiples of 16, so that none reads past p.columns
+  const int piece = n_tokens <= kExchange<kMode> ? kExchange<kMode> : kExchange<kMode> / 16 * 16;
+  for (int c0 = 0; c0 < n_tokens; c0 += piece) {
+    const int n = min(piece, n_tokens - c0);
     if (have) {
-      const int quadrant = warp & 3;
+      const int quadrant = warp & 3, groups = (n + 15) / 16;
       float* row = reinterpret_cast<float*>(sm) + quadrant * 32 + lane;
       const uint32_t at = tmem + (static_cast<uint32_t>(quadrant * 32) << 16) + c0;
-      for (int c = ((warp - 4) >> 2) * 16; c < n; c += 32) {
+#pragma unroll 1
+      for (int i = warp >> 2; i < (kDual ? 2 : 1) * groups; i += kNThreads / 128) {
+        const int part = i >= groups, c = (part ? i - groups : i) * 16;
+        __syncwarp();
+        uint32_t r[16];
+        tmem_ld16(at + part * p.columns + c, r);
+        tmem_wait_ld();
+        float* to = row + (part * kExchange<kMode> + c) * kNRows;
 #pragma unroll
-        for (int part = 0; part < (kDual ? 2 : 1); ++part) {
-          __syncwarp();
-          uint32_t r[16];
-          tmem_ld16(at + part * p.columns + c, r);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (c + e < kExchange<kMode>) row[(part * kExchange<kMode> + c + e) * kNRows] = __uint_as_float(r[e]);
-        }
+        for (int e = 0; e < 16; ++e)
+          if (c + e < kExchange<kMode>) to[e * kNRows] = __uint_as_float(r[e]);
       }
     }
     __syncthreads();
@@ -250,8 +257,8 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
           up = *reinterpret_cast<const uint2*>(p.up + token * p.up_stride + col);
         }
         Parts a, b;
-        a.load(partial, t, feature, ranks);
-        if (kDual) b.load(partial, kExchange<kMode> + t, feature, ranks);
+        a.load(partial, t, feature, ranks, rank);
+        if (kDual) b.load(partial, kExchange<kMode> + t, feature, ranks, rank);
         float v[4];
         a.sum(ranks, v);
         if (kDual) {
@@ -281,7 +288,7 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
     __syncthreads();
     cluster_barrier();  // no CTA leaves, or writes the next tokens' sums, while another reads these
   }
-  if (warp >= 4) tc_fence_before();
+  tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();

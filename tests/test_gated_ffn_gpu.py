@@ -107,6 +107,8 @@ SIZES = [
     (33, 1032, 264, 136),
     (64, 128, 4096, 64),
     (101, 256, 688, 256),
+    (110, 192, 264, 136),    # the first product exchanges its sums in two pieces
+    (126, 64, 392, 72),
     (128, 256, 512, 256),    # one full row tile
     (129, 320, 384, 264),    # one row past it
     (300, 512, 1368, 512),
