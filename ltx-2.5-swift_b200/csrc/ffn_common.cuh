@@ -90,7 +90,7 @@ struct NarrowParams {
   int tokens, features;
   int kb, kb_first;      // 64-wide K slices in all, and of the first pair
   int columns;           // tokens of a tile: a multiple of 16, the box of b
-  int tiles;             // feature tiles
+  int token_tiles;
   int stages;
   int follows;           // the kernel before it in the stream belongs to the same call
   int activation;
@@ -110,8 +110,13 @@ enum NarrowMode {
 
 constexpr int kNarrowColumns = 128;  // tokens of a tile at most
 
-// Tokens of a tile for a call of that many.
-inline int narrow_columns(int tokens) { return tokens >= kNarrowColumns ? kNarrowColumns : (int)div_up(tokens, 16) * 16; }
+// Tokens of a tile.  Where the features alone give few tiles, half the tokens: the CTAs that share a tile then
+// exchange half as much (101 tokens at 2048 x 5464: 35.5 -> 32.7 us; 128 at 4096 x 16384, whose first product has
+// 128 tiles without that: 89.5 -> 102.6).
+inline int narrow_columns(int tokens, int features) {
+  const int64_t tiles = div_up(tokens, kNarrowColumns) * (tokens > 48 && features <= 64 * 128 ? 2 : 1);
+  return (int)div_up(div_up(tokens, tiles), 16) * 16;
+}
 // Rows of the boxes of a[]: 128 features K-major, 64 of K MN-major.
 inline int narrow_box(NarrowMode mode) { return mode == kNarrowProduct || mode == kNarrowStore ? 128 : kFfnK; }
 // `follows`: the kernel before it in the stream belongs to the same call and does not write the weights.

@@ -126,8 +126,8 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank(), ranks = cluster_size();
   const int tile = blockIdx.x / ranks;
-  const int f0 = (tile % p.tiles) * kNRows;
-  const int t0 = (tile / p.tiles) * p.columns;
+  const int f0 = (tile / p.token_tiles) * kNRows;  // neighbours share weights
+  const int t0 = (tile % p.token_tiles) * p.columns;
   const int kb0 = (int)((int64_t)p.kb * rank / ranks), kb1 = (int)((int64_t)p.kb * (rank + 1) / ranks);
   const int kb_n = kb1 - kb0;  // >= 1: there are no more ranks than K slices
   const uint32_t stage_bytes = kWeights<kMode> + p.columns * kFfnK * 2;
@@ -299,66 +299,41 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
 constexpr int kMaxDev = 64;
 std::mutex g_mu;
 
-struct Occupancy {
-  bool ready;
-  int clusters[kNMaxCluster + 1];  // clusters of that size that run together
-};
-Occupancy g_occupancy[kMaxDev][4];
+bool g_ready[kMaxDev][4];
 
 template <NarrowMode kMode>
-cudaError_t prepare(Occupancy* out) {
+cudaError_t prepare() {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= kMaxDev) return cudaErrorInvalidDevice;
   std::lock_guard<std::mutex> lock(g_mu);
-  Occupancy& o = g_occupancy[dev][kMode];
-  if (!o.ready) {
-    e = cudaFuncSetAttribute(narrow_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(narrow_kernel<kMode>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                               cudaSharedmemCarveoutMaxShared);
-    if (e != cudaSuccess) return e;
-    for (int s = 1; s <= kNMaxCluster; ++s) {
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = s * 64;
-      cfg.blockDim = kNThreads;
-      cfg.dynamicSmemBytes = kNSmem;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = s;
-      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      e = cudaOccupancyMaxActiveClusters(&o.clusters[s], narrow_kernel<kMode>, &cfg);
-      if (e != cudaSuccess) return e;
-    }
-    o.ready = true;
-  }
-  *out = o;
-  return cudaSuccess;
+  if (g_ready[dev][kMode]) return cudaSuccess;
+  e = cudaFuncSetAttribute(narrow_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kNSmem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(narrow_kernel<kMode>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                             cudaSharedmemCarveoutMaxShared);
+  g_ready[dev][kMode] = e == cudaSuccess;
+  return e;
 }
 
-// CTAs that share a tile: as many as fit the GPU at once, two to an SM (the
-// occupancy query counts one, as for every kernel that allocates TMEM; two run),
-// and leave each CTA four K slices.  More CTAs keep more loads in flight -- the
-// bandwidth needs about 13 MB of them -- but from some 250 on the exchange costs
-// more than that gives.  For 19 tokens at 2048 x 8192, 2, 3 and 4 CTAs to a tile
-// of the first product took 35.3, 34.0 and 33.0 us for both; for one token at
-// 4096 x 16384, 4, 5, 6 and 8 of the second 81.9, 76.8, 75.0 and 77.6.
-int choose_cluster(const Occupancy& o, int64_t tiles, int kb) {
-  for (int s = std::min(kNMaxCluster, kb / 4); s > 1; --s)
-    if (tiles <= 2 * o.clusters[s] && tiles * s <= 256) return s;
-  return 1;
+// CTAs that share a tile: as many as the GPU holds at once (296, two to an SM;
+// clusters leave some places empty) with two K slices or more each.  More CTAs
+// keep more loads in flight, and the bandwidth needs about 13 MB of them; from
+// some 260 on the exchange costs more than that gives.  For 19 tokens at 2048 x
+// 8192, 2, 3 and 4 CTAs to a tile of the first product (64 tiles) took 32.3, 29.1
+// and 28.5 us for both products; for one token at 4096 x 16384, 4, 6 and 8 to a
+// tile of the second (32 tiles) 75.2, 69.1 and 68.9.
+int choose_cluster(int64_t tiles, int kb) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>({kNMaxCluster, kb / 2, 264 / tiles}));
 }
 
 template <NarrowMode kMode>
 int launch(NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
-  Occupancy o;
-  cudaError_t e = prepare<kMode>(&o);
+  cudaError_t e = prepare<kMode>();
   if (e == cudaSuccess) {
-    const int64_t tiles = (int64_t)p.tiles * div_up(p.tokens, p.columns);
-    const int cluster = choose_cluster(o, tiles, p.kb);
+    const int64_t tiles = div_up(p.features, kNRows) * p.token_tiles;
+    const int cluster = choose_cluster(tiles, p.kb);
     if (tiles * cluster > 0x7fffffff) return fail_ffn(LTXATTN_ERR_UNSUPPORTED, "%s: too many output tiles", call);
     p.stages = std::min<int>(kNMaxStages, kNStageSpace / (kWeights<kMode> + p.columns * kFfnK * 2));
     cudaLaunchConfig_t cfg = {};
@@ -387,7 +362,7 @@ int launch(NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
 }  // namespace
 
 int launch_narrow(NarrowMode mode, NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
-  p.tiles = (int)div_up(p.features, kNRows);
+  p.token_tiles = (int)div_up(p.tokens, p.columns);
   p.err = device_error_word();
   if (!p.err) return fail_ffn(LTXATTN_ERR_CUDA, "no device error word");
   switch (mode) {

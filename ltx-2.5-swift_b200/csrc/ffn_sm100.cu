@@ -474,7 +474,7 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
   if (a->m <= kNarrowTokens) {
     NarrowParams p{};
     p.tokens = a->m;
-    p.columns = narrow_columns(a->m);
+    p.columns = narrow_columns(a->m, a->inner);
     p.features = a->inner;
     p.kb = p.kb_first = (int)div_up(a->hidden, kFfnK);
     p.activation = a->activation;
@@ -492,7 +492,7 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
 
     NarrowParams d{};
     d.tokens = a->m;
-    d.columns = p.columns;
+    d.columns = narrow_columns(a->m, a->out_dim);
     d.features = a->out_dim;
     d.kb = d.kb_first = (int)div_up(a->inner, kFfnK);
     d.out = static_cast<__nv_bfloat16*>(a->out);
@@ -594,7 +594,7 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
   if (narrow) {
     NarrowParams p{};
     p.tokens = a->m;
-    p.columns = narrow_columns(a->m);
+    p.columns = narrow_columns(a->m, a->inner);
     p.features = a->inner;
     p.kb = p.kb_first = (int)div_up(a->out_dim, kFfnK);
     p.activation = a->activation;
@@ -613,7 +613,7 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     if (a->dx != nullptr) {
       NarrowParams d{};
       d.tokens = a->m;
-      d.columns = p.columns;
+      d.columns = narrow_columns(a->m, a->hidden);
       d.features = a->hidden;
       d.kb_first = (int)div_up(a->inner, kFfnK);
       d.kb = 2 * d.kb_first;
