@@ -70,6 +70,35 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
 }
 
 // ---------------------------------------------------------------------------
+// clusters
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+// Every thread of every CTA of the cluster comes here, whatever happened before:
+// a CTA whose wait gave up still arrives.  Shared memory written before is
+// visible to the cluster after.
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// The address that `local` has in this CTA, of the CTA with that rank (shared::cluster window).
+__device__ __forceinline__ uint32_t peer_address(uint32_t local, uint32_t rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+  return at;
+}
+
+// ---------------------------------------------------------------------------
 // host side
 
 // Records the message and gives the status back.

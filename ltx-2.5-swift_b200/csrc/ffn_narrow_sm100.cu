@@ -46,25 +46,6 @@ constexpr int kExchange = kNStageSpace / (kNRows * 4) / (kMode == kNarrowProduct
 template <NarrowMode kMode>
 constexpr uint32_t kWeights = kMode == kNarrowProduct ? 2 * kNATile : kNATile;
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-
-// Every thread of every CTA of the cluster comes here, whatever happened before:
-// a CTA whose wait gave up still arrives.  Shared memory written before is
-// visible to the cluster after.
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-}
-
 // 4 floats at the address that `local` has in this CTA, of the CTA with that rank (of this one: without the
 // way through the cluster's network, which gives some 10 bytes a cycle to an SM).
 __device__ __forceinline__ float4 peer_load4(uint32_t local, uint32_t rank, uint32_t own) {
@@ -76,11 +57,9 @@ __device__ __forceinline__ float4 peer_load4(uint32_t local, uint32_t rank, uint
                  : "memory");
     return v;
   }
-  uint32_t at;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(at)
+               : "r"(peer_address(local, rank))
                : "memory");
   return v;
 }

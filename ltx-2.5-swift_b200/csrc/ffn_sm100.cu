@@ -9,11 +9,14 @@
 //              dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
 //
 // One persistent kernel, gemm_kernel<A major, B major, epilogue>, makes them
-// all: a CTA per SM walks over 128 x 256 output tiles (fp32 in TMEM).  Warp 0
-// lane 0 loads 64-wide K slices of both operands with TMA into a ring of
-// shared-memory stages (128-byte swizzle), warp 1 lane 0 issues the MMAs, and
-// warps 4-11 turn the finished accumulator into the output while the next
-// tile's MMAs fill the other half of TMEM.
+// all.  A pair of CTAs (a cluster, cta_group::2) walks over 256 x 256 output
+// tiles: each holds 128 rows of A and 128 of B's 256 columns in its shared
+// memory, and 128 rows of the result in its TMEM, so an SM loads 32 KB for the
+// MMAs that one on its own would load 48 KB for.  In each CTA warp 0 lane 0
+// loads 64-wide K slices with TMA into a ring of stages (128-byte swizzle) that
+// the first CTA's barrier counts; there warp 1 lane 0 issues the MMAs for both;
+// warps 4-11 turn the finished accumulator into the output while the next tile's
+// MMAs fill the other half of TMEM.
 //
 // Operands that lie along the wrong axis (the weights of dh and dx, both
 // operands of the weight gradients) are read as they lie: their tiles are
@@ -42,20 +45,22 @@ int set_error_message(int status, const char* msg);
 
 namespace {
 
-constexpr int kGM = 128;       // rows of a tile (UMMA M)
+constexpr int kGM = 128;       // rows of a CTA's part of a tile
+constexpr int kGPairM = 2 * kGM;  // rows of a tile (UMMA M)
 constexpr int kGN = 256;       // accumulator columns of a tile (UMMA N)
+constexpr int kGHalfN = kGN / 2;  // of which a CTA holds the operand
 constexpr int kGK = kFfnK;
-constexpr int kGStages = 4;
+constexpr int kGStages = 6;
 constexpr int kGThreads = 384;  // 4 control warps, 8 epilogue warps
 constexpr uint32_t kGA = kGM * kGK * 2;
-constexpr uint32_t kGB = kGN * kGK * 2;
+constexpr uint32_t kGB = kGHalfN * kGK * 2;
 constexpr uint32_t kGStage = kGA + kGB;
 constexpr uint32_t kChunk = 64 * kGK * 2;  // MN-major: 64 columns x 64 rows of K
-// full[kGStages], empty[kGStages], acc_full[2], acc_empty[2]
+// full[kGStages] and acc_empty[2] (the first CTA's count for both), empty[kGStages], acc_full[2]
 constexpr uint32_t kGOffBar = kGStages * kGStage;
 constexpr uint32_t kGOffCtl = kGOffBar + (2 * kGStages + 4) * 8;  // TMEM slot, abort flag
 constexpr uint32_t kGSmem = kGOffCtl + 16 + 1024;                 // + alignment slack
-constexpr int kGEpilogueThreads = 256;
+constexpr int kGEpilogueWarps = 8;
 
 enum Epilogue { kProduct, kStore, kSlopes };
 
@@ -84,7 +89,7 @@ struct GemmParams {
 
 // Tiles are numbered down the rows first, in bands of kBand row blocks: the CTAs
 // that run together then share a few column blocks of B and the band's rows of A.
-constexpr int kBand = 16;
+constexpr int kBand = 8;
 
 __device__ __forceinline__ void locate(const GemmParams& p, int tile, int& which, int& m0, int& tn) {
   which = 0;
@@ -94,12 +99,52 @@ __device__ __forceinline__ void locate(const GemmParams& p, int tile, int& which
   const int band = i / (kBand * g.tiles_n);
   const int rows = min(kBand, g.tiles_m - band * kBand);
   const int j = i - band * kBand * g.tiles_n;
-  m0 = (band * kBand + j % rows) * kGM;
+  m0 = (band * kBand + j % rows) * kGPairM;
   tn = j / rows;
 }
 
+// TMEM and MMAs of a CTA pair.  Both CTAs allocate and free; the first one issues.
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t* slot, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(columns)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_free(uint32_t tmem, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+}
+__device__ __forceinline__ void pair_mma(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                         uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}\n" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives at `bar` of both CTAs once every MMA issued so far is done.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+// A load into this CTA's shared memory that is counted at a barrier of either CTA (its shared::cluster address).
+__device__ __forceinline__ void pair_load(const CUtensorMap* map, uint32_t bar, void* dst, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void cluster_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 template <bool kAMN, bool kBMN, int kEpilogue>
-__global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
+    gemm_kernel(const __grid_constant__ GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = align1024(smem_raw);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + kGOffBar);
@@ -109,32 +154,36 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + kGOffCtl);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + kGOffCtl + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank();
   const int tiles = p.first_tile[p.count];
+  const int first = blockIdx.x / 2, step = gridDim.x / 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * kGStages; ++i) mbar_init(full + i, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + i, 1);
-      mbar_init(acc_empty + i, kGEpilogueThreads / 32);
+      mbar_init(acc_empty + i, 2 * kGEpilogueWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
+  __syncwarp();
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+    pair_tmem_alloc(tmem_slot, 512);
     tc_fence_before();
   }
   __syncthreads();
+  cluster_barrier();  // both CTAs' barriers are set up
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0 && lane == 0) {
     int it = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+    for (int tile = first; tile < tiles && ok; tile += step) {
       int which, m0, tn;
       locate(p, tile, which, m0, tn);
+      m0 += rank * kGM;
       const Gemm& g = p.g[which];
       for (int kb = 0; kb < g.kb; ++kb, ++it) {
         const int st = it % kGStages, u = it / kGStages;
@@ -146,37 +195,38 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
         uint8_t* sb = sa + kGA;
         const int part = kb >= g.kb_first;
         const int k0 = (part ? kb - g.kb_first : kb) * kGK;
-        mbar_arrive_expect_tx(full + st, kGStage);
+        const uint32_t bar = peer_address(smem_u32(full + st), 0);
+        if (rank == 0) mbar_arrive_expect_tx(full + st, 2 * kGStage);
         if (kAMN) {
 #pragma unroll
-          for (int c = 0; c < kGM / 64; ++c) tma_load_2d(&g.a[part], full + st, sa + c * kChunk, m0 + c * 64, k0);
+          for (int c = 0; c < kGM / 64; ++c) pair_load(&g.a[part], bar, sa + c * kChunk, m0 + c * 64, k0);
         } else {
-          tma_load_2d(&g.a[part], full + st, sa, k0, m0);
+          pair_load(&g.a[part], bar, sa, k0, m0);
         }
         if (kEpilogue == kProduct) {
-          // rows 0-127 of the B tile are the gate's weights, rows 128-255 the up projection's
-          tma_load_2d(&g.b[0], full + st, sb, k0, tn * (kGN / 2));
-          tma_load_2d(&g.b[1], full + st, sb + kGB / 2, k0, tn * (kGN / 2));
+          // the first CTA's half of B is the gate's weights, the second's the up projection's
+          pair_load(&g.b[rank], bar, sb, k0, tn * kGHalfN);
         } else if (kBMN) {
 #pragma unroll
-          for (int c = 0; c < kGN / 64; ++c)
-            tma_load_2d(&g.b[part], full + st, sb + c * kChunk, tn * kGN + c * 64, k0);
+          for (int c = 0; c < kGHalfN / 64; ++c)
+            pair_load(&g.b[part], bar, sb + c * kChunk, tn * kGN + rank * kGHalfN + c * 64, k0);
         } else {
-          tma_load_2d(&g.b[part], full + st, sb, k0, tn * kGN);
+          pair_load(&g.b[part], bar, sb, k0, tn * kGN + rank * kGHalfN);
         }
       }
     }
-    // never leave the CTA with a bulk copy still writing its shared memory
-    for (int i = it < kGStages ? 0 : it - kGStages; i < it; ++i) drain_wait(full + i % kGStages, (i / kGStages) & 1);
-  } else if (warp == 1 && lane == 0) {
-    constexpr uint32_t idesc = idesc_bf16_f32(kGM, kGN, kAMN, kBMN);
+    // never leave the CTA with a bulk copy still writing its shared memory: a stage is empty again once it was
+    // full and has been read
+    for (int i = it < kGStages ? 0 : it - kGStages; i < it; ++i) drain_wait(empty + i % kGStages, (i / kGStages) & 1);
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    constexpr uint32_t idesc = idesc_bf16_f32(kGPairM, kGN, kAMN, kBMN);
     const SDesc a0 = sdesc_split(smem_u32(sm), kAMN ? kChunk : 16, 1024);
     const SDesc b0 = sdesc_split(smem_u32(sm) + kGA, kBMN ? kChunk : 16, 1024);
     // 16 of K further along: 32 bytes of each row K-major, 16 rows of 128 bytes MN-major
     constexpr uint32_t a_step = kAMN ? 128 : 2, b_step = kBMN ? 128 : 2;
     int it = 0, n = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
+    for (int tile = first; tile < tiles && ok; tile += step, ++n) {
       int which, m0, tn;
       locate(p, tile, which, m0, tn);
       const int kb_n = p.g[which].kb;
@@ -194,10 +244,10 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
         const uint32_t alo = a0.lo + st * (kGStage >> 4), blo = b0.lo + st * (kGStage >> 4);
 #pragma unroll
         for (int kk = 0; kk < kGK / 16; ++kk)
-          umma_ss2(d, alo + kk * a_step, a0.hi, blo + kk * b_step, b0.hi, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(empty + st);  // the stage is free once these MMAs have read it
+          pair_mma(d, alo + kk * a_step, a0.hi, blo + kk * b_step, b0.hi, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+        pair_commit(empty + st);  // the stage is free, in both CTAs, once these MMAs have read it
       }
-      umma_commit(acc_full + buf);
+      pair_commit(acc_full + buf);
     }
     // no MMA still running when the CTA tears down: the last commits cover all of them
     for (int i = n < 2 ? 0 : n - 2; i < n; ++i) drain_wait(acc_full + (i & 1), (i >> 1) & 1);
@@ -205,9 +255,10 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
     const int quadrant = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lane_off = static_cast<uint32_t>(quadrant * 32) << 16;
     int n = 0;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+    for (int tile = first; tile < tiles; tile += step, ++n) {
       int which, m0, tn;
       locate(p, tile, which, m0, tn);
+      m0 += rank * kGM;
       const Gemm& g = p.g[which];
       const int buf = n & 1;
       if (!warp_wait(acc_full + buf, (n >> 1) & 1, abort_flag, p.err, 64)) break;
@@ -219,12 +270,12 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
         // 64 columns of h per warp: accumulator columns c (gate) and 128 + c (up)
 #pragma unroll 1
         for (int c = half * 64; c < half * 64 + 64; c += 16) {
-          const int col = tn * (kGN / 2) + c;
+          const int col = tn * kGHalfN + c;
           if (col >= g.N) break;  // warp-uniform
           __syncwarp();
           uint32_t rg[16], ru[16];
           tmem_ld16(d + c, rg);
-          tmem_ld16(d + kGN / 2 + c, ru);
+          tmem_ld16(d + kGHalfN + c, ru);
           tmem_wait_ld();
           if (!exists) continue;
 #pragma unroll
@@ -277,14 +328,16 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty + buf);
+      if (lane == 0) cluster_arrive(peer_address(smem_u32(acc_empty + buf), 0));
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
+  cluster_barrier();  // neither CTA leaves while the other's MMAs or arrivals reach it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    pair_tmem_free(tmem, 512);
   }
 }
 
@@ -396,11 +449,11 @@ cudaError_t prepare_kernel(K kernel, int slot, int* sms) {
 
 template <bool kAMN, bool kBMN, int kEpilogue>
 int launch_gemm(GemmParams& p, int slot, const char* call, cudaStream_t st) {
-  const int width = kEpilogue == kProduct ? kGN / 2 : kGN;
+  const int width = kEpilogue == kProduct ? kGHalfN : kGN;
   int64_t tiles = 0;
   for (int i = 0; i < p.count; ++i) {
     Gemm& g = p.g[i];
-    g.tiles_m = (int)div_up(g.M, kGM);
+    g.tiles_m = (int)div_up(g.M, kGPairM);
     g.tiles_n = (int)div_up(g.N, width);
     p.first_tile[i] = (int)tiles;
     tiles += (int64_t)g.tiles_m * g.tiles_n;
@@ -413,7 +466,7 @@ int launch_gemm(GemmParams& p, int slot, const char* call, cudaStream_t st) {
   cudaError_t e = prepare_kernel(gemm_kernel<kAMN, kBMN, kEpilogue>, slot, &sms);
   if (e == cudaSuccess) {
     gemm_kernel<kAMN, kBMN, kEpilogue>
-        <<<(unsigned)std::min<int64_t>(tiles, sms), kGThreads, kGSmem, st>>>(p);
+        <<<2 * (unsigned)std::min<int64_t>(tiles, sms / 2), kGThreads, kGSmem, st>>>(p);
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) {
@@ -508,8 +561,8 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
   p.activation = a->activation;
   Gemm& g = p.g[0];
   if (int rc = ffn_map(&g.a[0], a->x, a->m, a->hidden, a->x_stride, kGM, "x")) return rc;
-  if (int rc = ffn_map(&g.b[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, kGN / 2, "w_gate")) return rc;
-  if (int rc = ffn_map(&g.b[1], a->w_up, a->inner, a->hidden, a->w_up_stride, kGN / 2, "w_up")) return rc;
+  if (int rc = ffn_map(&g.b[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, kGHalfN, "w_gate")) return rc;
+  if (int rc = ffn_map(&g.b[1], a->w_up, a->inner, a->hidden, a->w_up_stride, kGHalfN, "w_up")) return rc;
   g.M = a->m;
   g.N = a->inner;
   g.kb = g.kb_first = (int)div_up(a->hidden, kGK);
@@ -525,7 +578,7 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
   d.count = 1;
   Gemm& o = d.g[0];
   if (int rc = ffn_map(&o.a[0], h, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
-  if (int rc = ffn_map(&o.b[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, kGN, "w_down")) return rc;
+  if (int rc = ffn_map(&o.b[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, kGHalfN, "w_down")) return rc;
   o.M = a->m;
   o.N = a->out_dim;
   o.kb = o.kb_first = (int)div_up(a->inner, kGK);
