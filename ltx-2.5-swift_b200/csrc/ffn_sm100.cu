@@ -50,19 +50,32 @@ constexpr int kGPairM = 2 * kGM;  // rows of a tile (UMMA M)
 constexpr int kGN = 256;       // accumulator columns of a tile (UMMA N)
 constexpr int kGHalfN = kGN / 2;  // of which a CTA holds the operand
 constexpr int kGK = kFfnK;
-constexpr int kGStages = 6;
 constexpr int kGThreads = 384;  // 4 control warps, 8 epilogue warps
 constexpr uint32_t kGA = kGM * kGK * 2;
 constexpr uint32_t kGB = kGHalfN * kGK * 2;
 constexpr uint32_t kGStage = kGA + kGB;
 constexpr uint32_t kChunk = 64 * kGK * 2;  // MN-major: 64 columns x 64 rows of K
-// full[kGStages] and acc_empty[2] (the first CTA's count for both), empty[kGStages], acc_full[2]
-constexpr uint32_t kGOffBar = kGStages * kGStage;
-constexpr uint32_t kGOffCtl = kGOffBar + (2 * kGStages + 4) * 8;  // TMEM slot, abort flag
-constexpr uint32_t kGSmem = kGOffCtl + 16 + 1024;                 // + alignment slack
 constexpr int kGEpilogueWarps = 8;
 
 enum Epilogue { kProduct, kStore, kSlopes };
+
+// The epilogue's warps pass their 32 rows x 32 columns through shared memory, so that they are written (and the
+// kept gate and up read) as whole 64-byte pieces of rows: a thread finds a row in TMEM, and storing rows from
+// there takes a line of memory per thread and access.  Rows are padded to 80 (bf16) or 144 bytes (fp32), which
+// spreads eight of them over all banks.
+constexpr uint32_t kRowBf16 = 80, kRowF32 = 144;
+
+template <int kEpilogue>
+struct GemmSmem {
+  static constexpr int kStages = kEpilogue == kSlopes ? 5 : 6;
+  static constexpr uint32_t kRow = kEpilogue == kSlopes ? kRowF32 : kRowBf16;
+  static constexpr uint32_t kOffStaging = kStages * kGStage;
+  // full[kStages] (the first CTA's counts for both), empty[kStages], acc_full[2], acc_empty[2] (the first CTA's)
+  static constexpr uint32_t kOffBar = kOffStaging + 8 * 32 * kRow;
+  static constexpr uint32_t kOffCtl = kOffBar + (2 * kStages + 4) * 8;  // TMEM slot, abort flag
+  static constexpr uint32_t kBytes = kOffCtl + 16 + 1024;               // + alignment slack
+  static_assert(kBytes <= kMaxDynamicSmem, "shared memory of a CTA");
+};
 
 // One output of a launch (a launch of the weight gradients has up to three).
 struct Gemm {
@@ -142,17 +155,40 @@ __device__ __forceinline__ void cluster_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// 32 rows (one per lane) x 32 columns of the warp to bf16 rows of global memory, from `row0` and `col` on; what is
+// outside M x N is left out.
+__device__ __forceinline__ void flush(uint8_t* staging, int lane, const float (&v)[32], __nv_bfloat16* out,
+                                      int64_t stride, int64_t row0, int col, int M, int N) {
+  uint4* mine = reinterpret_cast<uint4*>(staging + lane * kRowBf16);
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    mine[q] = make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                         pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
+  __syncwarp();
+  const int piece = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = (lane >> 2) + 8 * i;
+    const uint4 w = *reinterpret_cast<const uint4*>(staging + r * kRowBf16 + piece * 16);
+    if (row0 + r < M && col + 8 * piece < N)
+      *reinterpret_cast<uint4*>(out + (row0 + r) * stride + col + 8 * piece) = w;
+  }
+  __syncwarp();
+}
+
 template <bool kAMN, bool kBMN, int kEpilogue>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
     gemm_kernel(const __grid_constant__ GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = align1024(smem_raw);
-  uint64_t* full = reinterpret_cast<uint64_t*>(sm + kGOffBar);
+  using S = GemmSmem<kEpilogue>;
+  constexpr int kGStages = S::kStages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + S::kOffBar);
   uint64_t* empty = full + kGStages;
   uint64_t* acc_full = empty + kGStages;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + kGOffCtl);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + kGOffCtl + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + S::kOffCtl);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + S::kOffCtl + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int tiles = p.first_tile[p.count];
@@ -176,6 +212,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
   cluster_barrier();  // both CTAs' barriers are set up
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  grid_dep_launch_dependents();
+  grid_dep_wait();  // all that is read may have been written by the kernel before
 
   if (warp == 0 && lane == 0) {
     int it = 0;
@@ -254,49 +292,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
   } else if (warp >= 4) {
     const int quadrant = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lane_off = static_cast<uint32_t>(quadrant * 32) << 16;
+    uint8_t* staging = sm + S::kOffStaging + (warp - 4) * 32 * S::kRow;
     int n = 0;
     for (int tile = first; tile < tiles; tile += step, ++n) {
       int which, m0, tn;
       locate(p, tile, which, m0, tn);
-      m0 += rank * kGM;
       const Gemm& g = p.g[which];
       const int buf = n & 1;
       if (!warp_wait(acc_full + buf, (n >> 1) & 1, abort_flag, p.err, 64)) break;
       tc_fence_after();
       const uint32_t d = tmem + buf * kGN + lane_off;
-      const int64_t row = m0 + quadrant * 32 + lane;
-      const bool exists = row < g.M;
-      if (kEpilogue == kProduct) {
+      const int64_t row0 = m0 + rank * kGM + quadrant * 32;
+      if (row0 >= g.M) {
+        // nothing of this warp's exists
+      } else if (kEpilogue == kProduct) {
         // 64 columns of h per warp: accumulator columns c (gate) and 128 + c (up)
 #pragma unroll 1
-        for (int c = half * 64; c < half * 64 + 64; c += 16) {
+        for (int c = half * 64; c < half * 64 + 64; c += 32) {
           const int col = tn * kGHalfN + c;
           if (col >= g.N) break;  // warp-uniform
           __syncwarp();
-          uint32_t rg[16], ru[16];
-          tmem_ld16(d + c, rg);
-          tmem_ld16(d + kGHalfN + c, ru);
+          uint32_t rg[32], ru[32];
+          tmem_ld32(d + c, rg);
+          tmem_ld32(d + kGHalfN + c, ru);
           tmem_wait_ld();
-          if (!exists) continue;
+          float v[32];
+          if (p.gate != nullptr) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            if (col + 8 * q >= g.N) break;
-            float v[8], gv[8], uv[8];
+            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(rg[e]);
+            flush(staging, lane, v, p.gate, p.gate_stride, row0, col, g.M, g.N);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              gv[e] = __uint_as_float(rg[8 * q + e]);
-              uv[e] = __uint_as_float(ru[8 * q + e]);
-              float unused;
-              v[e] = activate<false>(p.activation, gv[e], unused) * uv[e];
-            }
-            store8(g.out + row * g.out_stride + col + 8 * q, v);
-            if (p.gate != nullptr) {
-              store8(p.gate + row * p.gate_stride + col + 8 * q, gv);
-              store8(p.up + row * p.up_stride + col + 8 * q, uv);
-            }
+            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(ru[e]);
+            flush(staging, lane, v, p.up, p.up_stride, row0, col, g.M, g.N);
           }
+          float unused;
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            v[e] = activate<false>(p.activation, __uint_as_float(rg[e]), unused) * __uint_as_float(ru[e]);
+          flush(staging, lane, v, g.out, g.out_stride, row0, col, g.M, g.N);
         }
-      } else {
+      } else if (kEpilogue == kStore) {
 #pragma unroll 1
         for (int c = half * 128; c < half * 128 + 128; c += 32) {
           const int col = tn * kGN + c;
@@ -305,24 +340,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
           uint32_t r[32];
           tmem_ld32(d + c, r);
           tmem_wait_ld();
-          if (!exists) continue;
+          float v[32];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (col + 8 * q >= g.N) break;
-            float v[8];
+          for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
+          flush(staging, lane, v, g.out, g.out_stride, row0, col, g.M, g.N);
+        }
+      } else {
+        const int piece = lane & 3;
+#pragma unroll 1
+        for (int c = half * 128; c < half * 128 + 128; c += 32) {
+          const int col = tn * kGN + c;
+          if (col >= g.N) break;  // warp-uniform
+          // the kept gate and up, on their way while dh goes through shared memory
+          uint4 gw[4], uw[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[8 * q + e]);
-            if (kEpilogue == kSlopes) {
-              float gv[8], uv[8], dgv[8], duv[8];
-              load8(p.gate + row * p.gate_stride + col + 8 * q, gv);
-              load8(p.up + row * p.up_stride + col + 8 * q, uv);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) slopes(p.activation, gv[e], uv[e], v[e], dgv[e], duv[e], v[e]);
-              store8(p.dgate + row * p.dgate_stride + col + 8 * q, dgv);
-              store8(p.dup + row * p.dup_stride + col + 8 * q, duv);
-              if (g.out == nullptr) continue;  // h is wanted for dw_down alone
+          for (int i = 0; i < 4; ++i) {
+            const int64_t row = row0 + (lane >> 2) + 8 * i;
+            gw[i] = uw[i] = make_uint4(0, 0, 0, 0);
+            if (row < g.M && col + 8 * piece < g.N) {
+              gw[i] = *reinterpret_cast<const uint4*>(p.gate + row * p.gate_stride + col + 8 * piece);
+              uw[i] = *reinterpret_cast<const uint4*>(p.up + row * p.up_stride + col + 8 * piece);
             }
-            store8(g.out + row * g.out_stride + col + 8 * q, v);
+          }
+          __syncwarp();
+          uint32_t r[32];
+          tmem_ld32(d + c, r);
+          tmem_wait_ld();
+          uint4* mine = reinterpret_cast<uint4*>(staging + lane * kRowF32);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) mine[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rr = (lane >> 2) + 8 * i;
+            const float4* src = reinterpret_cast<const float4*>(staging + rr * kRowF32 + piece * 32);
+            const float4 lo = src[0], hi = src[1];
+            const float dh[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            float gv[8], uv[8], dgv[8], duv[8], hv[8];
+            unpack8(gw[i], gv);
+            unpack8(uw[i], uv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) slopes(p.activation, gv[e], uv[e], dh[e], dgv[e], duv[e], hv[e]);
+            const int64_t row = row0 + rr;
+            if (row < g.M && col + 8 * piece < g.N) {
+              store8(p.dgate + row * p.dgate_stride + col + 8 * piece, dgv);
+              store8(p.dup + row * p.dup_stride + col + 8 * piece, duv);
+              if (g.out != nullptr)  // h is wanted for dw_down alone
+                store8(g.out + row * g.out_stride + col + 8 * piece, hv);
+            }
           }
         }
       }
@@ -431,14 +496,14 @@ int g_sms[kMaxDev] = {};
 
 // The SM count, with the kernel's shared memory opted into once per device.
 template <typename K>
-cudaError_t prepare_kernel(K kernel, int slot, int* sms) {
+cudaError_t prepare_kernel(K kernel, int slot, uint32_t smem, int* sms) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= kMaxDev) return cudaErrorInvalidDevice;
   std::lock_guard<std::mutex> lock(g_mu);
   if (!g_attr_set[dev][slot]) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGSmem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
     g_attr_set[dev][slot] = true;
@@ -463,12 +528,11 @@ int launch_gemm(GemmParams& p, int slot, const char* call, cudaStream_t st) {
   p.err = device_error_word();
   if (!p.err) return fail_ffn(LTXATTN_ERR_CUDA, "no device error word");
   int sms = 0;
-  cudaError_t e = prepare_kernel(gemm_kernel<kAMN, kBMN, kEpilogue>, slot, &sms);
-  if (e == cudaSuccess) {
-    gemm_kernel<kAMN, kBMN, kEpilogue>
-        <<<2 * (unsigned)std::min<int64_t>(tiles, sms / 2), kGThreads, kGSmem, st>>>(p);
-    e = cudaGetLastError();
-  }
+  constexpr uint32_t smem = GemmSmem<kEpilogue>::kBytes;
+  cudaError_t e = prepare_kernel(gemm_kernel<kAMN, kBMN, kEpilogue>, slot, smem, &sms);
+  if (e == cudaSuccess)
+    e = launch_pdl(gemm_kernel<kAMN, kBMN, kEpilogue>, 2 * (unsigned)std::min<int64_t>(tiles, sms / 2), kGThreads, smem,
+                   st, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return fail_ffn(LTXATTN_ERR_CUDA, "%s: %s", call, cudaGetErrorString(e));
