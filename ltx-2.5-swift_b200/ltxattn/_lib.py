@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(HERE), "libltxattn_cuda.so")
@@ -180,6 +181,11 @@ class RotaryEmbedArgs(ctypes.Structure):
                 ("offset", ctypes.c_int64)]
 
 
+# The bytes of a RotaryEmbedArgs, field by field (native sizes and alignment, as the C compiler lays it out): for
+# callers that pack a call's arguments at once.
+ROTARY_EMBED_ARGS = struct.Struct("@9if" + 4 * "Pqqq" + "PPiqqq")
+
+
 def _rows(*names):
     return [f for n in names for f in ((n, ctypes.c_void_p), (n + "_stride", ctypes.c_int64))]
 
@@ -187,6 +193,11 @@ def _rows(*names):
 _FFN_SIZES = [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("m", ctypes.c_int32),
               ("hidden", ctypes.c_int32), ("inner", ctypes.c_int32), ("out_dim", ctypes.c_int32)]
 _WORKSPACE = [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+# The bytes of a GatedFfnArgs and of a GatedFfnBwdArgs.
+GATED_FFN_ARGS = struct.Struct("@6i" + 7 * "Pq" + "PN")
+GATED_FFN_BWD_ARGS = struct.Struct("@6i" + 11 * "Pq" + "PN")
 
 
 class GatedFfnArgs(ctypes.Structure):
@@ -269,12 +280,12 @@ def load(path: str = LIB_PATH):
     L.ltxattn_rotary_frequencies.argtypes = [ctypes.POINTER(RotaryFrequencyArgs), ctypes.POINTER(ctypes.c_double),
                                              ctypes.POINTER(ctypes.c_float)]
     L.ltxattn_rotary_frequencies.restype = ctypes.c_int
-    L.ltxattn_rotary_embed.argtypes = [ctypes.POINTER(RotaryEmbedArgs), vp]
+    L.ltxattn_rotary_embed.argtypes = [vp, vp]  # a struct by reference, or its bytes
     L.ltxattn_rotary_embed.restype = ctypes.c_int
-    for name, args in (("ltxattn_gated_ffn", GatedFfnArgs), ("ltxattn_gated_ffn_bwd", GatedFfnBwdArgs)):
-        getattr(L, name).argtypes = [ctypes.POINTER(args), vp]
+    for name in ("ltxattn_gated_ffn", "ltxattn_gated_ffn_bwd"):
+        getattr(L, name).argtypes = [vp, vp]
         getattr(L, name).restype = ctypes.c_int
-        getattr(L, name + "_workspace").argtypes = [ctypes.POINTER(args)]
+        getattr(L, name + "_workspace").argtypes = [vp]
         getattr(L, name + "_workspace").restype = ctypes.c_size_t
     L.ltxattn_abi_version.argtypes = []
     L.ltxattn_abi_version.restype = ctypes.c_int

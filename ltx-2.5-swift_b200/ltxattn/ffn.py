@@ -7,7 +7,6 @@ bf16, fp32 accumulation; the product between the projections is rounded once.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional
 
@@ -21,6 +20,10 @@ ACTIVATIONS = {"silu": 0, "gelu_tanh": 1, "gelu": 2}
 
 def _matrix(name: str, t: torch.Tensor, rows: int, cols: int, device: int) -> tuple:
     """(address, row stride) of a bf16 [rows, cols] matrix on that device."""
+    if isinstance(t, torch.Tensor) and t.shape == (rows, cols) and t.dtype == torch.bfloat16 and t.get_device() == device:
+        stride, unit = t.stride()
+        if unit == 1 or cols <= 1:
+            return t.data_ptr(), stride if rows > 1 else cols
     _check_cuda(name, t)
     if t.dtype != torch.bfloat16:
         raise Failure("dtype", f"{name} must be bfloat16", _lib.ERR_DTYPE)
@@ -28,10 +31,7 @@ def _matrix(name: str, t: torch.Tensor, rows: int, cols: int, device: int) -> tu
         raise Failure.shape(name, t.shape, f"[{rows}, {cols}]")
     if t.get_device() != device:
         raise Failure("arg", f"{name} is on {t.device}, the tokens on cuda:{device}", _lib.ERR_ARG)
-    stride, unit = t.stride()
-    if unit != 1 and cols > 1:
-        raise Failure("align", f"{name} must have a unit stride along its last dim", _lib.ERR_ALIGN)
-    return t.data_ptr(), stride if rows > 1 else cols
+    raise Failure("align", f"{name} must have a unit stride along its last dim", _lib.ERR_ALIGN)
 
 
 def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -48,14 +48,10 @@ def _activation(name: str) -> int:
 def _output(name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor):
     """An output of that shape: the caller's, or a new one on the device of ``like``."""
     if t is None:
-        return like.new_empty(shape, dtype=torch.bfloat16)
+        return like.new_empty(shape) if like.dtype == torch.bfloat16 else like.new_empty(shape, dtype=torch.bfloat16)
     if t.shape != tuple(shape):
         raise Failure.shape(name, t.shape, str(list(shape)))
     return t
-
-
-def _workspace(need: int, like: torch.Tensor) -> Optional[torch.Tensor]:
-    return like.new_empty((need,), dtype=torch.uint8) if need else None
 
 
 def _out_rows(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -90,22 +86,20 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         x2 = _rows("x", x)
         m, hidden = x2.shape
         y = _output("out", out, lead + (out_dim,), x)
-        a = _lib.GatedFfnArgs(_lib.BF16, act, m, hidden, inner, out_dim, *_matrix("x", x2, m, hidden, device),
-                              *_matrix("w_gate", w_gate, inner, hidden, device),
-                              *_matrix("w_up", w_up, inner, hidden, device),
-                              *_matrix("w_down", w_down, out_dim, inner, device),
-                              *_matrix("out", _out_rows("out", y), m, out_dim, device))
         gate = up = None
+        kept = (0, 0, 0, 0)
         if save:
-            gate = x.new_empty(lead + (inner,))
+            gate = _output("gate", None, lead + (inner,), x)
             up = torch.empty_like(gate)
-            a.gate, a.gate_stride, a.up, a.up_stride = gate.data_ptr(), inner, up.data_ptr(), inner
-        L = _lib.load()
-        need = L.ltxattn_gated_ffn_workspace(ctypes.byref(a))
-        ws = _workspace(need, x)
-        if ws is not None:
-            a.workspace, a.workspace_bytes = ws.data_ptr(), need
-        rc = L.ltxattn_gated_ffn(ctypes.byref(a), st)
+            kept = (gate.data_ptr(), inner, up.data_ptr(), inner)
+        args = (_lib.BF16, act, m, hidden, inner, out_dim, *_matrix("x", x2, m, hidden, device),
+                *_matrix("w_gate", w_gate, inner, hidden, device), *_matrix("w_up", w_up, inner, hidden, device),
+                *_matrix("w_down", w_down, out_dim, inner, device),
+                *_matrix("out", _out_rows("out", y), m, out_dim, device), *kept)
+        L, pack = _lib.load(), _lib.GATED_FFN_ARGS.pack
+        need = L.ltxattn_gated_ffn_workspace(pack(*args, 0, 0))
+        ws = x.new_empty((need,), dtype=torch.uint8) if need else None
+        rc = L.ltxattn_gated_ffn(pack(*args, ws.data_ptr() if need else 0, need), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
     return (y, gate, up) if save else y
@@ -143,41 +137,27 @@ def gated_ffn_backward(x: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: to
     with _on(device, stream) as st:
         d2 = _rows("dout", dout)
         m, out_dim = d2.shape
-        a = _lib.GatedFfnBwdArgs(_lib.BF16, act, m, hidden, inner, out_dim)
-
-        def put(name, t, rows, cols):
-            ptr, stride = _matrix(name, t, rows, cols, device)
-            setattr(a, name, ptr)
-            setattr(a, name + "_stride", stride)
-
-        if x is not None:
-            put("x", _rows("x", x), m, hidden)
-        put("w_gate", w_gate, inner, hidden)
-        put("w_up", w_up, inner, hidden)
-        put("w_down", w_down, out_dim, inner)
-        put("gate", _rows("gate", gate), m, inner)
-        put("up", _rows("up", up), m, inner)
-        put("dout", d2, m, out_dim)
+        x2, gate2, up2 = (None if t is None else _rows(name, t) for name, t in (("x", x), ("gate", gate), ("up", up)))
         if need_dx:
             dx = _output("dx", dx, tuple(lead) + (hidden,), dout)
-            put("dx", _out_rows("dx", dx), m, hidden)
-        else:
-            dx = None
         if need_dw:
             dw_gate = _output("dw_gate", dw_gate, (inner, hidden), dout)
             dw_up = _output("dw_up", dw_up, (inner, hidden), dout)
             dw_down = _output("dw_down", dw_down, (out_dim, inner), dout)
-            put("dw_gate", dw_gate, inner, hidden)
-            put("dw_up", dw_up, inner, hidden)
-            put("dw_down", dw_down, out_dim, inner)
-        else:
-            dw_gate = dw_up = dw_down = None
-        L = _lib.load()
-        need = L.ltxattn_gated_ffn_bwd_workspace(ctypes.byref(a))
-        ws = _workspace(need, dout)
-        if ws is not None:
-            a.workspace, a.workspace_bytes = ws.data_ptr(), need
-        rc = L.ltxattn_gated_ffn_bwd(ctypes.byref(a), st)
+        nothing = (0, 0)
+        args = (_lib.BF16, act, m, hidden, inner, out_dim,
+                *(nothing if x2 is None else _matrix("x", x2, m, hidden, device)),
+                *_matrix("w_gate", w_gate, inner, hidden, device), *_matrix("w_up", w_up, inner, hidden, device),
+                *_matrix("w_down", w_down, out_dim, inner, device), *_matrix("gate", gate2, m, inner, device),
+                *_matrix("up", up2, m, inner, device), *_matrix("dout", d2, m, out_dim, device),
+                *(_matrix("dx", _out_rows("dx", dx), m, hidden, device) if need_dx else nothing),
+                *(_matrix("dw_gate", dw_gate, inner, hidden, device) if need_dw else nothing),
+                *(_matrix("dw_up", dw_up, inner, hidden, device) if need_dw else nothing),
+                *(_matrix("dw_down", dw_down, out_dim, inner, device) if need_dw else nothing))
+        L, pack = _lib.load(), _lib.GATED_FFN_BWD_ARGS.pack
+        need = L.ltxattn_gated_ffn_bwd_workspace(pack(*args, 0, 0))
+        ws = dout.new_empty((need,), dtype=torch.uint8) if need else None
+        rc = L.ltxattn_gated_ffn_bwd(pack(*args, ws.data_ptr() if need else 0, need), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
-    return dx, dw_gate, dw_up, dw_down
+    return (dx if need_dx else None,) + ((dw_gate, dw_up, dw_down) if need_dw else (None, None, None))

@@ -33,6 +33,19 @@ def test_ctypes_layout_matches_the_header(tmp_path):
     assert got == want
 
 
+@pytest.mark.parametrize("packer,py", [(_lib.ROTARY_EMBED_ARGS, _lib.RotaryEmbedArgs),
+                                       (_lib.GATED_FFN_ARGS, _lib.GatedFfnArgs),
+                                       (_lib.GATED_FFN_BWD_ARGS, _lib.GatedFfnBwdArgs)])
+def test_packed_arguments_are_the_struct(packer, py):
+    def flat(c):  # every scalar field, in order
+        return [x for n, t in c._fields_ for x in (flat(getattr(c, n)) if isinstance(getattr(c, n), ctypes.Structure)
+                                                   else [getattr(c, n)])]
+
+    assert packer.size == ctypes.sizeof(py)
+    values = list(range(1, len(flat(py())) + 1))
+    assert flat(py.from_buffer_copy(packer.pack(*values))) == values
+
+
 # ---- frequencies ----
 
 def table(*args, **kw):
