@@ -145,6 +145,8 @@ inline int narrow_columns(int tokens, int features) {
   const int64_t tiles = div_up(tokens, kNarrowColumns) * (tokens > 48 && features <= 64 * 128 ? 2 : 1);
   return (int)div_up(div_up(tokens, tiles), 16) * 16;
 }
+// What a product is expected to take, in microseconds.
+double narrow_us(NarrowMode mode, int tokens, int features, int kb);
 // Rows of the boxes of a[]: 128 features K-major, 64 of K MN-major.
 inline int narrow_box(NarrowMode mode) { return mode == kNarrowProduct || mode == kNarrowStore ? 128 : kFfnK; }
 // `follows`: the kernel before it in the stream belongs to the same call and does not write the weights.

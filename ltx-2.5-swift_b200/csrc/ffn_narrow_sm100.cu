@@ -130,7 +130,6 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  grid_dep_launch_dependents();
 
   if (warp == 0 && lane == 0) {
     auto weights = [&](int i) {
@@ -158,9 +157,12 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
     // The second product of a call need not wait for the first to load its weights, only to load its tokens.
     // The first one waits for whatever was before it in the stream, which may have written anything.
     const int first = min(stages, kb_n);
+    // The kernel after this one may start once this wait is over in every CTA, so what came before this call is
+    // complete when it loads its weights.
     if (!p.follows) grid_dep_wait();
     for (int i = 0; i < first; ++i) weights(i);
     if (p.follows) grid_dep_wait();
+    grid_dep_launch_dependents();
     for (int i = 0; i < first; ++i) tokens(i);
     int i = first;
     for (; i < kb_n; ++i) {
@@ -339,6 +341,18 @@ int launch(NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
 }
 
 }  // namespace
+
+// Rounds of up to 296 CTAs; an SM brings in 1 KB of a slice per 11 ns for the one or two CTAs that it holds, and 1 KB
+// of another CTA's sums per 34 ns.
+double narrow_us(NarrowMode mode, int tokens, int features, int kb) {
+  const int columns = narrow_columns(tokens, features), parts = mode == kNarrowProduct ? 2 : 1;
+  const int64_t tiles = div_up(features, kNRows) * div_up(tokens, columns);
+  const int cluster = choose_cluster(tiles, kb);
+  const int64_t ctas = tiles * cluster, rounds = div_up(ctas, 296);
+  const double on_sm = ctas > 148 ? 2.0 * rounds : 1.0;
+  const double slice_kb = parts * 16 + columns / 8.0, exchange_kb = columns * parts * 0.5 * (cluster - 1) / cluster;
+  return 5.5 * rounds + on_sm * (0.011 * div_up(kb, cluster) * slice_kb + 0.034 * exchange_kb);
+}
 
 int launch_narrow(NarrowMode mode, NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
   p.token_tiles = (int)div_up(p.tokens, p.columns);

@@ -212,8 +212,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
   cluster_barrier();  // both CTAs' barriers are set up
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  grid_dep_launch_dependents();
   grid_dep_wait();  // all that is read may have been written by the kernel before
+  grid_dep_launch_dependents();
 
   if (warp == 0 && lane == 0) {
     int it = 0;
@@ -540,8 +540,16 @@ int launch_gemm(GemmParams& p, int slot, const char* call, cudaStream_t st) {
   return LTXATTN_OK;
 }
 
-// Up to this many tokens the products run feature by feature (ffn_narrow_sm100.cu).
-constexpr int kNarrowTokens = 128;
+// Whether a product runs feature by feature (ffn_narrow_sm100.cu), by what both kernels were measured to take: 106
+// shapes of 24 to 2000 tokens and 256 to 16384 features gave the constants here and there.  The rule's choice is on
+// average 1.5% slower than the faster kernel; choosing by 128 or 256 tokens 20% and 10%.  The wide kernel pays for
+// rounds of tiles over 74 CTA pairs, which few tokens leave mostly empty: at 320 tokens and 1024 x 2816 the forward's
+// products take 23 us feature by feature and 35 here, at 512 and 4096 x 16384 265 and 200.
+bool few_tokens(int tokens, int features, int kb, NarrowMode mode) {
+  const int64_t tiles = div_up(tokens, kGPairM) * div_up(features, mode == kNarrowProduct ? kGHalfN : kGN);
+  const double wide_us = 6.5 + (double)div_up(tiles, 74) * (0.31 * kb + 2.8);
+  return narrow_us(mode, tokens, features, kb) < wide_us;
+}
 
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
@@ -588,12 +596,13 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   __nv_bfloat16* h = static_cast<__nv_bfloat16*>(a->workspace);
 
-  if (a->m <= kNarrowTokens) {
+  const int kb_in = (int)div_up(a->hidden, kFfnK), kb_out = (int)div_up(a->inner, kFfnK);
+  if (few_tokens(a->m, a->inner, kb_in, kNarrowProduct)) {
     NarrowParams p{};
     p.tokens = a->m;
     p.columns = narrow_columns(a->m, a->inner);
     p.features = a->inner;
-    p.kb = p.kb_first = (int)div_up(a->hidden, kFfnK);
+    p.kb = p.kb_first = kb_in;
     p.activation = a->activation;
     p.out = h;
     p.out_stride = a->inner;
@@ -606,49 +615,49 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
     if (int rc = ffn_map(&p.a[1], a->w_up, a->inner, a->hidden, a->w_up_stride, box, "w_up")) return rc;
     if (int rc = ffn_map(&p.b[0], a->x, a->m, a->hidden, a->x_stride, p.columns, "x")) return rc;
     if (int rc = launch_narrow(kNarrowProduct, p, false, call, st)) return rc;
-
-    NarrowParams d{};
-    d.tokens = a->m;
-    d.columns = narrow_columns(a->m, a->out_dim);
-    d.features = a->out_dim;
-    d.kb = d.kb_first = (int)div_up(a->inner, kFfnK);
-    d.out = static_cast<__nv_bfloat16*>(a->out);
-    d.out_stride = a->out_stride;
-    if (int rc = ffn_map(&d.a[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, narrow_box(kNarrowStore), "w_down"))
-      return rc;
-    if (int rc = ffn_map(&d.b[0], h, a->m, a->inner, a->inner, d.columns, "workspace")) return rc;
-    return launch_narrow(kNarrowStore, d, true, call, st);
+  } else {
+    GemmParams p{};
+    p.count = 1;
+    p.activation = a->activation;
+    Gemm& g = p.g[0];
+    if (int rc = ffn_map(&g.a[0], a->x, a->m, a->hidden, a->x_stride, kGM, "x")) return rc;
+    if (int rc = ffn_map(&g.b[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, kGHalfN, "w_gate")) return rc;
+    if (int rc = ffn_map(&g.b[1], a->w_up, a->inner, a->hidden, a->w_up_stride, kGHalfN, "w_up")) return rc;
+    g.M = a->m;
+    g.N = a->inner;
+    g.kb = g.kb_first = kb_in;
+    g.out = h;
+    g.out_stride = a->inner;
+    p.gate = static_cast<__nv_bfloat16*>(a->gate);
+    p.up = static_cast<__nv_bfloat16*>(a->up);
+    p.gate_stride = a->gate_stride;
+    p.up_stride = a->up_stride;
+    if (int rc = launch_gemm<false, false, kProduct>(p, 0, call, st)) return rc;
   }
-
+  if (few_tokens(a->m, a->out_dim, kb_out, kNarrowStore)) {
+    NarrowParams p{};
+    p.tokens = a->m;
+    p.columns = narrow_columns(a->m, a->out_dim);
+    p.features = a->out_dim;
+    p.kb = p.kb_first = kb_out;
+    p.out = static_cast<__nv_bfloat16*>(a->out);
+    p.out_stride = a->out_stride;
+    if (int rc = ffn_map(&p.a[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, narrow_box(kNarrowStore), "w_down"))
+      return rc;
+    if (int rc = ffn_map(&p.b[0], h, a->m, a->inner, a->inner, p.columns, "workspace")) return rc;
+    return launch_narrow(kNarrowStore, p, true, call, st);
+  }
   GemmParams p{};
   p.count = 1;
-  p.activation = a->activation;
   Gemm& g = p.g[0];
-  if (int rc = ffn_map(&g.a[0], a->x, a->m, a->hidden, a->x_stride, kGM, "x")) return rc;
-  if (int rc = ffn_map(&g.b[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, kGHalfN, "w_gate")) return rc;
-  if (int rc = ffn_map(&g.b[1], a->w_up, a->inner, a->hidden, a->w_up_stride, kGHalfN, "w_up")) return rc;
+  if (int rc = ffn_map(&g.a[0], h, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
+  if (int rc = ffn_map(&g.b[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, kGHalfN, "w_down")) return rc;
   g.M = a->m;
-  g.N = a->inner;
-  g.kb = g.kb_first = (int)div_up(a->hidden, kGK);
-  g.out = h;
-  g.out_stride = a->inner;
-  p.gate = static_cast<__nv_bfloat16*>(a->gate);
-  p.up = static_cast<__nv_bfloat16*>(a->up);
-  p.gate_stride = a->gate_stride;
-  p.up_stride = a->up_stride;
-  if (int rc = launch_gemm<false, false, kProduct>(p, 0, call, st)) return rc;
-
-  GemmParams d{};
-  d.count = 1;
-  Gemm& o = d.g[0];
-  if (int rc = ffn_map(&o.a[0], h, a->m, a->inner, a->inner, kGM, "workspace")) return rc;
-  if (int rc = ffn_map(&o.b[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, kGHalfN, "w_down")) return rc;
-  o.M = a->m;
-  o.N = a->out_dim;
-  o.kb = o.kb_first = (int)div_up(a->inner, kGK);
-  o.out = static_cast<__nv_bfloat16*>(a->out);
-  o.out_stride = a->out_stride;
-  return launch_gemm<false, false, kStore>(d, 1, call, st);
+  g.N = a->out_dim;
+  g.kb = g.kb_first = kb_out;
+  g.out = static_cast<__nv_bfloat16*>(a->out);
+  g.out_stride = a->out_stride;
+  return launch_gemm<false, false, kStore>(p, 1, call, st);
 }
 
 size_t ltxattn_gated_ffn_bwd_workspace(const ltxattn_gated_ffn_bwd_args* a) {
@@ -706,14 +715,14 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
 
   __nv_bfloat16* gate = static_cast<__nv_bfloat16*>(const_cast<void*>(a->gate));
   __nv_bfloat16* up = static_cast<__nv_bfloat16*>(const_cast<void*>(a->up));
-  const bool narrow = a->m <= kNarrowTokens;
-  // dh = dout w_down, and what follows from it element by element; then dx
-  if (narrow) {
+  const int kb_dh = (int)div_up(a->out_dim, kFfnK), kb_inner = (int)div_up(a->inner, kFfnK);
+  // dh = dout w_down, and what follows from it element by element
+  if (few_tokens(a->m, a->inner, kb_dh, kNarrowSlopes)) {
     NarrowParams p{};
     p.tokens = a->m;
     p.columns = narrow_columns(a->m, a->inner);
     p.features = a->inner;
-    p.kb = p.kb_first = (int)div_up(a->out_dim, kFfnK);
+    p.kb = p.kb_first = kb_dh;
     p.activation = a->activation;
     p.out = a->dw_down != nullptr ? h : nullptr;
     p.out_stride = p.dgate_stride = p.dup_stride = a->inner;
@@ -727,22 +736,6 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
       return rc;
     if (int rc = ffn_map(&p.b[0], a->dout, a->m, a->out_dim, a->dout_stride, p.columns, "dout")) return rc;
     if (int rc = launch_narrow(kNarrowSlopes, p, false, call, st)) return rc;
-    if (a->dx != nullptr) {
-      NarrowParams d{};
-      d.tokens = a->m;
-      d.columns = narrow_columns(a->m, a->hidden);
-      d.features = a->hidden;
-      d.kb_first = (int)div_up(a->inner, kFfnK);
-      d.kb = 2 * d.kb_first;
-      d.out = static_cast<__nv_bfloat16*>(a->dx);
-      d.out_stride = a->dx_stride;
-      const int box = narrow_box(kNarrowStoreMN);
-      if (int rc = ffn_map(&d.a[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, box, "w_gate")) return rc;
-      if (int rc = ffn_map(&d.a[1], a->w_up, a->inner, a->hidden, a->w_up_stride, box, "w_up")) return rc;
-      if (int rc = ffn_map(&d.b[0], dgate, a->m, a->inner, a->inner, d.columns, "workspace")) return rc;
-      if (int rc = ffn_map(&d.b[1], dup, a->m, a->inner, a->inner, d.columns, "workspace")) return rc;
-      if (int rc = launch_narrow(kNarrowStoreMN, d, true, call, st)) return rc;
-    }
   } else {
     GemmParams p{};
     p.count = 1;
@@ -752,7 +745,7 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     if (int rc = ffn_map(&g.b[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, kGK, "w_down")) return rc;
     g.M = a->m;
     g.N = a->inner;
-    g.kb = g.kb_first = (int)div_up(a->out_dim, kGK);
+    g.kb = g.kb_first = kb_dh;
     g.out = a->dw_down != nullptr ? h : nullptr;
     g.out_stride = a->inner;
     p.gate = gate;
@@ -764,7 +757,22 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     p.dgate_stride = p.dup_stride = a->inner;
     if (int rc = launch_gemm<false, true, kSlopes>(p, 2, call, st)) return rc;
   }
-  if (!narrow && a->dx != nullptr) {
+  if (a->dx != nullptr && few_tokens(a->m, a->hidden, 2 * kb_inner, kNarrowStoreMN)) {
+    NarrowParams p{};
+    p.tokens = a->m;
+    p.columns = narrow_columns(a->m, a->hidden);
+    p.features = a->hidden;
+    p.kb = 2 * kb_inner;
+    p.kb_first = kb_inner;
+    p.out = static_cast<__nv_bfloat16*>(a->dx);
+    p.out_stride = a->dx_stride;
+    const int box = narrow_box(kNarrowStoreMN);
+    if (int rc = ffn_map(&p.a[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, box, "w_gate")) return rc;
+    if (int rc = ffn_map(&p.a[1], a->w_up, a->inner, a->hidden, a->w_up_stride, box, "w_up")) return rc;
+    if (int rc = ffn_map(&p.b[0], dgate, a->m, a->inner, a->inner, p.columns, "workspace")) return rc;
+    if (int rc = ffn_map(&p.b[1], dup, a->m, a->inner, a->inner, p.columns, "workspace")) return rc;
+    if (int rc = launch_narrow(kNarrowStoreMN, p, true, call, st)) return rc;
+  } else if (a->dx != nullptr) {
     GemmParams p{};
     p.count = 1;
     Gemm& g = p.g[0];
@@ -774,8 +782,8 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     if (int rc = ffn_map(&g.b[1], a->w_up, a->inner, a->hidden, a->w_up_stride, kGK, "w_up")) return rc;
     g.M = a->m;
     g.N = a->hidden;
-    g.kb_first = (int)div_up(a->inner, kGK);
-    g.kb = 2 * g.kb_first;
+    g.kb = 2 * kb_inner;
+    g.kb_first = kb_inner;
     g.out = static_cast<__nv_bfloat16*>(a->dx);
     g.out_stride = a->dx_stride;
     if (int rc = launch_gemm<false, true, kStore>(p, 3, call, st)) return rc;

@@ -50,7 +50,7 @@ struct RotaryEmbedParams {
   int rows;          // B * T
   int slots;         // slots of a token: turned ones, then copied ones
   int turn_slots;    // pairs / kP
-  int slot_lanes, head_lanes;  // a CTA's threads
+  int slot_lanes, head_lanes, token_lanes;  // a CTA's threads
   const double* freq;
   const void* positions;  // or null: token t stands at t
   int pos64;
@@ -162,32 +162,37 @@ struct Slot {
   }
 };
 
-// A CTA takes one token with all its heads.  Its threads first make the token's
-// cos and sin, into shared memory; then thread (slot, head lane) keeps its
-// slot's in registers and walks over every head_lanes-th head of q and of k.
-// The heads of a token lie side by side in a projection's output, so a CTA
-// streams whole rows of it.  Many small CTAs keep the memory busy better than
-// more runs per thread: 128 threads at 48 registers take 150 us for
-// 29760 tokens x 64 heads x 128 in bf16 (6.5 TB/s, 0.99 of the measured copy);
-// fetching a head ahead of the one that turns 158, four heads at once 257.
+// A CTA takes token_lanes tokens (one, unless its heads are few) with all their
+// heads.  Its threads first make the tokens' cos and sin, into shared memory;
+// then thread (slot, head lane, token) keeps its slot's in registers and walks
+// over every head_lanes-th head of q and of k.  The heads of a token lie side by
+// side in a projection's output, so a CTA streams whole rows of it.  Many small
+// CTAs keep the memory busy better than more runs per thread: 128 threads at 48
+// registers take 150 us for 29760 tokens x 64 heads x 128 in bf16 (6.5 TB/s, 0.99
+// of the measured copy); fetching a head ahead of the one that turns 158, four
+// heads at once 257.
 template <typename T, int kP, bool kInterleaved>
 __global__ void __launch_bounds__(kRThreads, 5) rotary_embed_kernel(const __grid_constant__ RotaryEmbedParams p) {
-  extern __shared__ float2 turns[];  // [pairs]: (cos, sin), with the magnitude
-  const int64_t b = blockIdx.x / p.T, t = blockIdx.x - b * p.T;
-  int64_t place = t;
-  if (p.positions != nullptr) {
-    const int64_t o = b * p.pos_sb + t * p.pos_st;
-    place = p.pos64 ? static_cast<const int64_t*>(p.positions)[o] : static_cast<const int32_t*>(p.positions)[o];
-  }
-  const double position = static_cast<double>(place + p.offset);
-  for (int j = threadIdx.x; j < p.pairs; j += blockDim.x) {
+  extern __shared__ float2 turns[];  // [token_lanes][pairs]: (cos, sin), with the magnitude
+  const int row0 = blockIdx.x * p.token_lanes;
+  const int n_rows = min(p.token_lanes, p.rows - row0);
+  for (int i = threadIdx.x; i < n_rows * p.pairs; i += blockDim.x) {
+    const int r = i / p.pairs, j = i - r * p.pairs;
+    const int64_t b = (row0 + r) / p.T, t = (row0 + r) - b * p.T;
+    int64_t place = t;
+    if (p.positions != nullptr) {
+      const int64_t o = b * p.pos_sb + t * p.pos_st;
+      place = p.pos64 ? static_cast<const int64_t*>(p.positions)[o] : static_cast<const int32_t*>(p.positions)[o];
+    }
     float c, s;
-    turn(position, p.freq[j], c, s);
-    turns[j] = make_float2(c * p.magnitude, p.inverse ? -s * p.magnitude : s * p.magnitude);
+    turn(static_cast<double>(place + p.offset), p.freq[j], c, s);
+    turns[i] = make_float2(c * p.magnitude, p.inverse ? -s * p.magnitude : s * p.magnitude);
   }
   __syncthreads();
   using S = Slot<T, kP, kInterleaved>;
-  const int h0 = threadIdx.x / p.slot_lanes;
+  const int rest = threadIdx.x / p.slot_lanes, r = rest / p.head_lanes, h0 = rest - r * p.head_lanes;
+  if (r >= n_rows) return;
+  const int64_t b = (row0 + r) / p.T, t = (row0 + r) - b * p.T;
   for (int slot = threadIdx.x % p.slot_lanes; slot < p.slots; slot += p.slot_lanes) {
     S w;
     w.turned = slot < p.turn_slots;
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(kRThreads, 5) rotary_embed_kernel(const __grid
     w.at = w.turned ? (kInterleaved ? 2 * kP : kP) * slot : 2 * p.pairs + S::kRun * (slot - p.turn_slots);
 #pragma unroll
     for (int e = 0; e < kP; ++e) {
-      const float2 cs = w.turned ? turns[slot * kP + e] : make_float2(1.f, 0.f);
+      const float2 cs = w.turned ? turns[r * p.pairs + slot * kP + e] : make_float2(1.f, 0.f);
       w.c[e] = cs.x;
       w.s[e] = cs.y;
     }
@@ -215,9 +220,9 @@ int fail_rotary(int status, const char* fmt, ...) {
 
 template <typename T, int kP>
 void launch(const RotaryEmbedParams& p, bool interleaved, cudaStream_t st) {
-  const unsigned grid = (unsigned)p.rows;
-  const int threads = p.slot_lanes * p.head_lanes;
-  const size_t smem = sizeof(float2) * p.pairs;
+  const unsigned grid = (unsigned)((p.rows + (int64_t)p.token_lanes - 1) / p.token_lanes);
+  const int threads = p.slot_lanes * p.head_lanes * p.token_lanes;
+  const size_t smem = sizeof(float2) * p.token_lanes * p.pairs;
   if (interleaved)
     rotary_embed_kernel<T, kP, true><<<grid, threads, smem, st>>>(p);
   else
@@ -373,6 +378,7 @@ int ltxattn_rotary_embed(const ltxattn_rotary_embed_args* a, void* stream) {
   p.inverse = a->inverse != 0;
   p.slot_lanes = std::min(p.slots, kRThreads);
   p.head_lanes = std::max(1, std::min((int)std::max(H, Hk), kTargetThreads / p.slot_lanes));
+  p.token_lanes = std::max(1, kTargetThreads / (p.slot_lanes * p.head_lanes));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (bf16) {
     switch (kp) {
