@@ -406,8 +406,9 @@ typedef enum ltxattn_activation {
  *    aligned; hidden, inner and out_dim multiples of 8; any m >= 0.
  *  - gate, up: both NULL, or [m, inner] outputs that keep x w_gate^T and
  *    x w_up^T (rounded to bf16) for the gradient.
- *  - workspace: ltxattn_gated_ffn_workspace() bytes, 256-byte aligned; it holds
- *    the product act(..) * (..) in bf16 between the two kernels. */
+ *  - workspace: ltxattn_gated_ffn_workspace() bytes, 256-byte aligned: the
+ *    product act(..) * (..) in bf16 between the two kernels, 2 m inner bytes
+ *    rounded up to 256. */
 typedef struct ltxattn_gated_ffn_args {
   int32_t dtype; /* LTXATTN_BF16 */
   int32_t activation;
@@ -448,7 +449,8 @@ LTXATTN_API size_t ltxattn_gated_ffn_workspace(const ltxattn_gated_ffn_args* arg
  * [out_dim, inner] may be NULL, and is then not computed (frozen weights).
  * x is read for dw_gate and dw_up alone, w_gate and w_up for dx alone: they may
  * be NULL where those are.  Layout rules as for ltxattn_gated_ffn; with m = 0
- * the weight gradients are set to zero.  Outputs must not overlap inputs or one
+ * the weight gradients are set to zero.  The workspace holds dgate, dup and h:
+ * three times the forward's bytes.  Outputs must not overlap inputs or one
  * another. */
 typedef struct ltxattn_gated_ffn_bwd_args {
   int32_t dtype; /* LTXATTN_BF16 */

@@ -54,12 +54,24 @@ def _output(name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor):
     return t
 
 
+def _planes(n: int, m: int, inner: int, like: torch.Tensor) -> torch.Tensor:
+    """A workspace of n bf16 [m, inner] planes, as ltxattn_gated_ffn_workspace counts them (asking it would take
+    another packing of the arguments)."""
+    return like.new_empty((n * ((2 * m * inner + 255) // 256 * 256),), dtype=torch.uint8)
+
+
 def _out_rows(name: str, t: torch.Tensor) -> torch.Tensor:
     """The same for an output, of which a copy is no use."""
     rows = _rows(name, t)
     if rows.numel() and rows.data_ptr() != t.data_ptr():
         raise Failure("align", f"{name}'s leading dims must collapse into rows of one stride", _lib.ERR_ALIGN)
     return rows
+
+
+def _first_dim(name: str, w: torch.Tensor) -> int:
+    if not isinstance(w, torch.Tensor) or w.dim() != 2:
+        raise Failure.shape(name, getattr(w, "shape", ()), "a matrix")
+    return w.shape[0]
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
@@ -77,15 +89,13 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if x.dim() < 1:
         raise Failure.shape("x", x.shape, "[..., hidden]")
     device = x.get_device()
-    for name, w in (("w_gate", w_gate), ("w_down", w_down)):
-        if not isinstance(w, torch.Tensor) or w.dim() != 2:
-            raise Failure.shape(name, getattr(w, "shape", ()), "a matrix")
-    inner, out_dim = w_gate.shape[0], w_down.shape[0]
+    inner, out_dim = _first_dim("w_gate", w_gate), _first_dim("w_down", w_down)
     lead = x.shape[:-1]
     with _on(device, stream) as st:
         x2 = _rows("x", x)
         m, hidden = x2.shape
-        y = _output("out", out, lead + (out_dim,), x)
+        y = torch.empty_like(x) if out is None and out_dim == hidden and x.is_contiguous() else \
+            _output("out", out, lead + (out_dim,), x)
         gate = up = None
         kept = (0, 0, 0, 0)
         if save:
@@ -95,11 +105,10 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         args = (_lib.BF16, act, m, hidden, inner, out_dim, *_matrix("x", x2, m, hidden, device),
                 *_matrix("w_gate", w_gate, inner, hidden, device), *_matrix("w_up", w_up, inner, hidden, device),
                 *_matrix("w_down", w_down, out_dim, inner, device),
-                *_matrix("out", _out_rows("out", y), m, out_dim, device), *kept)
-        L, pack = _lib.load(), _lib.GATED_FFN_ARGS.pack
-        need = L.ltxattn_gated_ffn_workspace(pack(*args, 0, 0))
-        ws = x.new_empty((need,), dtype=torch.uint8) if need else None
-        rc = L.ltxattn_gated_ffn(pack(*args, ws.data_ptr() if need else 0, need), st)
+                *((y.data_ptr(), out_dim) if out is None else _matrix("out", _out_rows("out", y), m, out_dim, device)),
+                *kept)
+        ws = _planes(1, m, inner, x)
+        rc = _lib.load().ltxattn_gated_ffn(_lib.GATED_FFN_ARGS.pack(*args, ws.data_ptr(), ws.numel()), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
     return (y, gate, up) if save else y
@@ -154,10 +163,8 @@ def gated_ffn_backward(x: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: to
                 *(_matrix("dw_gate", dw_gate, inner, hidden, device) if need_dw else nothing),
                 *(_matrix("dw_up", dw_up, inner, hidden, device) if need_dw else nothing),
                 *(_matrix("dw_down", dw_down, out_dim, inner, device) if need_dw else nothing))
-        L, pack = _lib.load(), _lib.GATED_FFN_BWD_ARGS.pack
-        need = L.ltxattn_gated_ffn_bwd_workspace(pack(*args, 0, 0))
-        ws = dout.new_empty((need,), dtype=torch.uint8) if need else None
-        rc = L.ltxattn_gated_ffn_bwd(pack(*args, ws.data_ptr() if need else 0, need), st)
+        ws = _planes(3, m, inner, dout)
+        rc = _lib.load().ltxattn_gated_ffn_bwd(_lib.GATED_FFN_BWD_ARGS.pack(*args, ws.data_ptr(), ws.numel()), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
     return (dx if need_dx else None,) + ((dw_gate, dw_up, dw_down) if need_dw else (None, None, None))
