@@ -4,6 +4,7 @@
 
 #include <cstdio>
 #include <mutex>
+#include <type_traits>
 
 #include "../../include/ltxattn.h"
 #include "ltxattn_internal.h"
@@ -18,14 +19,13 @@ namespace ltx {
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
 // act(g), and with kSlope its derivative too.
-template <bool kSlope>
-__device__ __forceinline__ float activate(int kind, float g, float& slope) {
-  if (kind == LTXATTN_SILU) {
+template <int kAct, bool kSlope>
+__device__ __forceinline__ float activate(float g, float& slope) {
+  if constexpr (kAct == LTXATTN_SILU) {
     const float s = sigmoid(g);
     if (kSlope) slope = s * fmaf(g, 1.0f - s, 1.0f);
     return g * s;
-  }
-  if (kind == LTXATTN_GELU_TANH) {
+  } else if constexpr (kAct == LTXATTN_GELU_TANH) {
     // (1 + tanh z) / 2 = sigmoid(2 z)
     constexpr float c2 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
     const float g2 = g * g;
@@ -35,19 +35,33 @@ __device__ __forceinline__ float activate(int kind, float g, float& slope) {
       slope = t == 0.0f ? s : fmaf(t, c2 * fmaf(0.134145f, g2, 1.0f), s);
     }
     return g * s;
+  } else {
+    const float s = 0.5f * erfcf(-0.70710678118654752f * g);
+    if (kSlope) slope = fmaf(g, 0.3989422804014327f * __expf(-0.5f * g * g), s);
+    return g * s;
   }
-  const float s = 0.5f * erfcf(-0.70710678118654752f * g);
-  if (kSlope) slope = fmaf(g, 0.3989422804014327f * __expf(-0.5f * g * g), s);
-  return g * s;
+}
+
+// Calls f with the activation as a constant.  One branch for the many elements that f handles: with one in every
+// element the gradient's epilogue took longer than its MMAs (47 thousand cycles a tile for 33).
+template <typename F>
+__device__ __forceinline__ void with_activation(int kind, F&& f) {
+  if (kind == LTXATTN_SILU)
+    f(std::integral_constant<int, LTXATTN_SILU>{});
+  else if (kind == LTXATTN_GELU_TANH)
+    f(std::integral_constant<int, LTXATTN_GELU_TANH>{});
+  else
+    f(std::integral_constant<int, LTXATTN_GELU>{});
 }
 
 __device__ __forceinline__ float lo_f(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_f(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
 // The gradient through act(g) * u from dh: (dg, du), and the product itself.
-__device__ __forceinline__ void slopes(int kind, float g, float u, float dh, float& dg, float& du, float& h) {
+template <int kAct>
+__device__ __forceinline__ void slopes(float g, float u, float dh, float& dg, float& du, float& h) {
   float slope;
-  const float a = activate<true>(kind, g, slope);
+  const float a = activate<kAct, true>(g, slope);
   dg = dh * u * slope;
   du = dh * a;
   h = a * u;
@@ -118,6 +132,7 @@ struct NarrowParams {
   int tokens, features;
   int kb, kb_first;      // 64-wide K slices in all, and of the first pair
   int columns;           // tokens of a tile: a multiple of 16, the box of b
+  int cluster;           // CTAs that share a tile
   int token_tiles;
   int stages;
   int follows;           // the kernel before it in the stream belongs to the same call
@@ -136,17 +151,12 @@ enum NarrowMode {
   kNarrowStoreMN   // dx = dg Wg + du Wu, weights MN-major
 };
 
-constexpr int kNarrowColumns = 128;  // tokens of a tile at most
-
-// Tokens of a tile.  Where the features alone give few tiles, half the tokens: the CTAs that share a tile then
-// exchange half as much (101 tokens at 2048 x 5464: 35.5 -> 32.7 us; 128 at 4096 x 16384, whose first product has
-// 128 tiles without that: 89.5 -> 102.6).
-inline int narrow_columns(int tokens, int features) {
-  const int64_t tiles = div_up(tokens, kNarrowColumns) * (tokens > 48 && features <= 64 * 128 ? 2 : 1);
-  return (int)div_up(div_up(tokens, tiles), 16) * 16;
-}
-// What a product is expected to take, in microseconds.
-double narrow_us(NarrowMode mode, int tokens, int features, int kb);
+// How such a product is cut: tokens of a tile, CTAs that share a tile, and what it is expected to take.
+struct NarrowPlan {
+  int columns, cluster;
+  double us;
+};
+NarrowPlan plan_narrow(NarrowMode mode, int tokens, int features, int kb);
 // Rows of the boxes of a[]: 128 features K-major, 64 of K MN-major.
 inline int narrow_box(NarrowMode mode) { return mode == kNarrowProduct || mode == kNarrowStore ? 128 : kFfnK; }
 // `follows`: the kernel before it in the stream belongs to the same call and does not write the weights.

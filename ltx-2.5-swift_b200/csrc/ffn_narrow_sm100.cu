@@ -30,6 +30,7 @@ constexpr int kNThreads = 256;  // 8 warps: a producer, an MMA issuer, and then 
 constexpr int kNRows = 128;     // features of a tile (UMMA M)
 constexpr int kNMaxStages = 6;
 constexpr int kNMaxCluster = 8;
+constexpr int kNarrowColumns = 128;  // tokens of a tile at most
 constexpr uint32_t kNATile = kNRows * kFfnK * 2;
 constexpr uint32_t kNChunk = 64 * kFfnK * 2;  // MN-major: 64 features x 64 rows of K
 constexpr uint32_t kNStageSpace = 108 * 1024;  // two CTAs to an SM
@@ -249,16 +250,20 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
             store4(p.gate + token * p.gate_stride + col, v);
             store4(p.up + token * p.up_stride + col, u);
           }
-          float unused;
+          with_activation(p.activation, [&](auto act) {
+            float unused;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = activate<false>(p.activation, v[e], unused) * u[e];
+            for (int e = 0; e < 4; ++e) v[e] = activate<decltype(act)::value, false>(v[e], unused) * u[e];
+          });
         }
         if (kMode == kNarrowSlopes) {
           float g[4], u[4], dg[4], du[4];
           unpack4(gate, g);
           unpack4(up, u);
+          with_activation(p.activation, [&](auto act) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) slopes(p.activation, g[e], u[e], v[e], dg[e], du[e], v[e]);
+            for (int e = 0; e < 4; ++e) slopes<decltype(act)::value>(g[e], u[e], v[e], dg[e], du[e], v[e]);
+          });
           store4(p.dgate + token * p.dgate_stride + col, dg);
           store4(p.dup + token * p.dup_stride + col, du);
           if (p.out == nullptr) continue;  // h is wanted for dw_down alone
@@ -298,23 +303,12 @@ cudaError_t prepare() {
   return e;
 }
 
-// CTAs that share a tile: as many as the GPU holds at once (296, two to an SM;
-// clusters leave some places empty) with two K slices or more each.  More CTAs
-// keep more loads in flight, and the bandwidth needs about 13 MB of them; from
-// some 260 on the exchange costs more than that gives.  For 19 tokens at 2048 x
-// 8192, 2, 3 and 4 CTAs to a tile of the first product (64 tiles) took 32.3, 29.1
-// and 28.5 us for both products; for one token at 4096 x 16384, 4, 6 and 8 to a
-// tile of the second (32 tiles) 75.2, 69.1 and 68.9.
-int choose_cluster(int64_t tiles, int kb) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>({kNMaxCluster, kb / 2, 264 / tiles}));
-}
-
 template <NarrowMode kMode>
 int launch(NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
   cudaError_t e = prepare<kMode>();
   if (e == cudaSuccess) {
     const int64_t tiles = div_up(p.features, kNRows) * p.token_tiles;
-    const int cluster = choose_cluster(tiles, p.kb);
+    const int cluster = p.cluster;
     if (tiles * cluster > 0x7fffffff) return fail_ffn(LTXATTN_ERR_UNSUPPORTED, "%s: too many output tiles", call);
     p.stages = std::min<int>(kNMaxStages, kNStageSpace / (kWeights<kMode> + p.columns * kFfnK * 2));
     cudaLaunchConfig_t cfg = {};
@@ -342,16 +336,41 @@ int launch(NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
 
 }  // namespace
 
-// Rounds of up to 296 CTAs; an SM brings in 1 KB of a slice per 11 ns for the one or two CTAs that it holds, and 1 KB
-// of another CTA's sums per 34 ns.
-double narrow_us(NarrowMode mode, int tokens, int features, int kb) {
-  const int columns = narrow_columns(tokens, features), parts = mode == kNarrowProduct ? 2 : 1;
-  const int64_t tiles = div_up(features, kNRows) * div_up(tokens, columns);
-  const int cluster = choose_cluster(tiles, kb);
-  const int64_t ctas = tiles * cluster, rounds = div_up(ctas, 296);
-  const double on_sm = ctas > 148 ? 2.0 * rounds : 1.0;
-  const double slice_kb = parts * 16 + columns / 8.0, exchange_kb = columns * parts * 0.5 * (cluster - 1) / cluster;
-  return 5.5 * rounds + on_sm * (0.011 * div_up(kb, cluster) * slice_kb + 0.034 * exchange_kb);
+// How many CTAs of clusters of that size the GPU holds at once, two to an SM: clusters stay within a GPC, and leave
+// some of the 296 places empty.
+constexpr int kPlaces[kNMaxCluster + 1] = {0, 296, 296, 270, 264, 260, 264, 210, 240};
+
+// What a cut takes, in microseconds: 5.5 a call's share and 3 a round of CTAs; an SM brings in 1 KB of a K slice per
+// 10 ns, and 1 KB of another CTA's sums per 28 ns, for the one or two CTAs that it holds; and all weights come in at
+// 6.4 TB/s.  Fitted to 2700 cuts of 128 products (96 to 1024 tokens, 1024 to 16384 features): the cut that it finds
+// fastest is 0.8 us slower than the fastest one measured, on average.
+double cut_us(int parts, int tokens, int features, int kb, int columns, int cluster) {
+  const int64_t ctas = div_up(features, kNRows) * div_up(tokens, columns) * cluster;
+  const int64_t rounds = ctas / kPlaces[cluster], rest = ctas - rounds * kPlaces[cluster];
+  const double cta = 0.0103 * div_up(kb, cluster) * (parts * 16 + columns / 8.0) +
+                     0.0285 * columns * parts * 0.5 * (cluster - 1) / cluster +
+                     (cluster > 1 && columns * parts > 208 ? 1.5 : 0.0);  // the exchange in two pieces
+  double us = 2.5 + rounds * (3.0 + 2 * cta);
+  if (rest > 0) us += 3.0 + cta * (rest > 148 ? 2.0 : 1.0 + rest / 148.0);
+  return std::max(us, 5.5 + 2e-5 * features * parts * kb);
+}
+
+// The fastest cut: token tiles as few as fit (128 columns each) or up to three more, 1 to 8 CTAs to a tile with a
+// K slice each.  More token tiles exchange less but load the weights more often from L2; more CTAs to a tile keep
+// more loads in flight but exchange more.
+NarrowPlan plan_narrow(NarrowMode mode, int tokens, int features, int kb) {
+  const int parts = mode == kNarrowProduct ? 2 : 1;
+  const int64_t least = div_up(tokens, kNarrowColumns);
+  NarrowPlan best{0, 0, 0};
+  for (int64_t t = least; t <= least + 3; ++t) {
+    const int columns = (int)div_up(div_up(tokens, t), 16) * 16;
+    for (int s = 1; s <= std::min(kNMaxCluster, kb); ++s) {
+      const double us = cut_us(parts, tokens, features, kb, columns, s);
+      if (best.cluster == 0 || us < best.us) best = {columns, s, us};
+    }
+    if (columns == 16) break;
+  }
+  return best;
 }
 
 int launch_narrow(NarrowMode mode, NarrowParams& p, bool follows, const char* call, cudaStream_t st) {

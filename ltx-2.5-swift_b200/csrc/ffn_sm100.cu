@@ -215,7 +215,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
   grid_dep_wait();  // all that is read may have been written by the kernel before
   grid_dep_launch_dependents();
 
-  if (warp == 0 && lane == 0) {
+  // warp 0 loads A, warp 2 B: one thread takes about as long to issue both loads' copies as the MMAs of a stage run
+  if ((warp == 0 || warp == 2) && lane == 0) {
     int it = 0;
     bool ok = true;
     for (int tile = first; tile < tiles && ok; tile += step) {
@@ -234,14 +235,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
         const int part = kb >= g.kb_first;
         const int k0 = (part ? kb - g.kb_first : kb) * kGK;
         const uint32_t bar = peer_address(smem_u32(full + st), 0);
-        if (rank == 0) mbar_arrive_expect_tx(full + st, 2 * kGStage);
-        if (kAMN) {
+        if (warp == 0) {
+          if (rank == 0) mbar_arrive_expect_tx(full + st, 2 * kGStage);
+          if (kAMN) {
 #pragma unroll
-          for (int c = 0; c < kGM / 64; ++c) pair_load(&g.a[part], bar, sa + c * kChunk, m0 + c * 64, k0);
-        } else {
-          pair_load(&g.a[part], bar, sa, k0, m0);
-        }
-        if (kEpilogue == kProduct) {
+            for (int c = 0; c < kGM / 64; ++c) pair_load(&g.a[part], bar, sa + c * kChunk, m0 + c * 64, k0);
+          } else {
+            pair_load(&g.a[part], bar, sa, k0, m0);
+          }
+        } else if (kEpilogue == kProduct) {
           // the first CTA's half of B is the gate's weights, the second's the up projection's
           pair_load(&g.b[rank], bar, sb, k0, tn * kGHalfN);
         } else if (kBMN) {
@@ -299,10 +301,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
       locate(p, tile, which, m0, tn);
       const Gemm& g = p.g[which];
       const int buf = n & 1;
+      const int64_t row0 = m0 + rank * kGM + quadrant * 32;
+      // 4 lanes to a row of 32 columns, in the order that flush() writes
+      const int piece = lane & 3;
+      uint4 gw[4], uw[4];  // kSlopes: the kept gate and up of the next 32 columns
+      auto fetch = [&](int c) {
+        const int col = tn * kGN + c + 8 * piece;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t row = row0 + (lane >> 2) + 8 * i;
+          gw[i] = uw[i] = make_uint4(0, 0, 0, 0);
+          if (row < g.M && col < g.N) {
+            gw[i] = *reinterpret_cast<const uint4*>(p.gate + row * p.gate_stride + col);
+            uw[i] = *reinterpret_cast<const uint4*>(p.up + row * p.up_stride + col);
+          }
+        }
+      };
+      if (kEpilogue == kSlopes) fetch(half * 128);
       if (!warp_wait(acc_full + buf, (n >> 1) & 1, abort_flag, p.err, 64)) break;
       tc_fence_after();
       const uint32_t d = tmem + buf * kGN + lane_off;
-      const int64_t row0 = m0 + rank * kGM + quadrant * 32;
       if (row0 >= g.M) {
         // nothing of this warp's exists
       } else if (kEpilogue == kProduct) {
@@ -325,10 +343,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
             for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(ru[e]);
             flush(staging, lane, v, p.up, p.up_stride, row0, col, g.M, g.N);
           }
-          float unused;
+          with_activation(p.activation, [&](auto act) {
+            float unused;
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            v[e] = activate<false>(p.activation, __uint_as_float(rg[e]), unused) * __uint_as_float(ru[e]);
+            for (int e = 0; e < 32; ++e)
+              v[e] = activate<decltype(act)::value, false>(__uint_as_float(rg[e]), unused) * __uint_as_float(ru[e]);
+          });
           flush(staging, lane, v, g.out, g.out_stride, row0, col, g.M, g.N);
         }
       } else if (kEpilogue == kStore) {
@@ -346,49 +366,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
           flush(staging, lane, v, g.out, g.out_stride, row0, col, g.M, g.N);
         }
       } else {
-        const int piece = lane & 3;
 #pragma unroll 1
         for (int c = half * 128; c < half * 128 + 128; c += 32) {
           const int col = tn * kGN + c;
           if (col >= g.N) break;  // warp-uniform
-          // the kept gate and up, on their way while dh goes through shared memory
-          uint4 gw[4], uw[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int64_t row = row0 + (lane >> 2) + 8 * i;
-            gw[i] = uw[i] = make_uint4(0, 0, 0, 0);
-            if (row < g.M && col + 8 * piece < g.N) {
-              gw[i] = *reinterpret_cast<const uint4*>(p.gate + row * p.gate_stride + col + 8 * piece);
-              uw[i] = *reinterpret_cast<const uint4*>(p.up + row * p.up_stride + col + 8 * piece);
-            }
-          }
           __syncwarp();
           uint32_t r[32];
           tmem_ld32(d + c, r);
           tmem_wait_ld();
+          uint4 now_g[4], now_u[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) now_g[i] = gw[i], now_u[i] = uw[i];
+          if (c + 32 < half * 128 + 128) fetch(c + 32);
           uint4* mine = reinterpret_cast<uint4*>(staging + lane * kRowF32);
 #pragma unroll
           for (int q = 0; q < 8; ++q) mine[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
           __syncwarp();
+          with_activation(p.activation, [&](auto act) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rr = (lane >> 2) + 8 * i;
-            const float4* src = reinterpret_cast<const float4*>(staging + rr * kRowF32 + piece * 32);
-            const float4 lo = src[0], hi = src[1];
-            const float dh[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-            float gv[8], uv[8], dgv[8], duv[8], hv[8];
-            unpack8(gw[i], gv);
-            unpack8(uw[i], uv);
+            for (int i = 0; i < 4; ++i) {
+              const int rr = (lane >> 2) + 8 * i;
+              const float4* src = reinterpret_cast<const float4*>(staging + rr * kRowF32 + piece * 32);
+              const float4 lo = src[0], hi = src[1];
+              const float dh[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+              float gv[8], uv[8], dgv[8], duv[8], hv[8];
+              unpack8(now_g[i], gv);
+              unpack8(now_u[i], uv);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) slopes(p.activation, gv[e], uv[e], dh[e], dgv[e], duv[e], hv[e]);
-            const int64_t row = row0 + rr;
-            if (row < g.M && col + 8 * piece < g.N) {
-              store8(p.dgate + row * p.dgate_stride + col + 8 * piece, dgv);
-              store8(p.dup + row * p.dup_stride + col + 8 * piece, duv);
-              if (g.out != nullptr)  // h is wanted for dw_down alone
-                store8(g.out + row * g.out_stride + col + 8 * piece, hv);
+              for (int e = 0; e < 8; ++e) slopes<decltype(act)::value>(gv[e], uv[e], dh[e], dgv[e], duv[e], hv[e]);
+              const int64_t row = row0 + rr;
+              if (row < g.M && col + 8 * piece < g.N) {
+                store8(p.dgate + row * p.dgate_stride + col + 8 * piece, dgv);
+                store8(p.dup + row * p.dup_stride + col + 8 * piece, duv);
+                if (g.out != nullptr)  // h is wanted for dw_down alone
+                  store8(g.out + row * g.out_stride + col + 8 * piece, hv);
+              }
             }
-          }
+          });
         }
       }
       tc_fence_before();
@@ -540,15 +554,18 @@ int launch_gemm(GemmParams& p, int slot, const char* call, cudaStream_t st) {
   return LTXATTN_OK;
 }
 
-// Whether a product runs feature by feature (ffn_narrow_sm100.cu), by what both kernels were measured to take: 106
-// shapes of 24 to 2000 tokens and 256 to 16384 features gave the constants here and there.  The rule's choice is on
-// average 1.5% slower than the faster kernel; choosing by 128 or 256 tokens 20% and 10%.  The wide kernel pays for
-// rounds of tiles over 74 CTA pairs, which few tokens leave mostly empty: at 320 tokens and 1024 x 2816 the forward's
-// products take 23 us feature by feature and 35 here, at 512 and 4096 x 16384 265 and 200.
-bool few_tokens(int tokens, int features, int kb, NarrowMode mode) {
+// Whether a product runs feature by feature (ffn_narrow_sm100.cu), by what both kernels were measured to take.  The
+// wide kernel pays for rounds of tiles over 74 CTA pairs, which few tokens leave mostly empty.
+bool few_tokens(int tokens, int features, int kb, NarrowMode mode, NarrowParams& p) {
+  const NarrowPlan plan = plan_narrow(mode, tokens, features, kb);
   const int64_t tiles = div_up(tokens, kGPairM) * div_up(features, mode == kNarrowProduct ? kGHalfN : kGN);
   const double wide_us = 6.5 + (double)div_up(tiles, 74) * (0.31 * kb + 2.8);
-  return narrow_us(mode, tokens, features, kb) < wide_us;
+  p.tokens = tokens;
+  p.features = features;
+  p.kb = p.kb_first = kb;
+  p.columns = plan.columns;
+  p.cluster = plan.cluster;
+  return plan.us < wide_us;
 }
 
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -597,24 +614,19 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
   __nv_bfloat16* h = static_cast<__nv_bfloat16*>(a->workspace);
 
   const int kb_in = (int)div_up(a->hidden, kFfnK), kb_out = (int)div_up(a->inner, kFfnK);
-  if (few_tokens(a->m, a->inner, kb_in, kNarrowProduct)) {
-    NarrowParams p{};
-    p.tokens = a->m;
-    p.columns = narrow_columns(a->m, a->inner);
-    p.features = a->inner;
-    p.kb = p.kb_first = kb_in;
-    p.activation = a->activation;
-    p.out = h;
-    p.out_stride = a->inner;
-    p.gate = static_cast<__nv_bfloat16*>(a->gate);
-    p.up = static_cast<__nv_bfloat16*>(a->up);
-    p.gate_stride = a->gate_stride;
-    p.up_stride = a->up_stride;
+  if (NarrowParams q{}; few_tokens(a->m, a->inner, kb_in, kNarrowProduct, q)) {
+    q.activation = a->activation;
+    q.out = h;
+    q.out_stride = a->inner;
+    q.gate = static_cast<__nv_bfloat16*>(a->gate);
+    q.up = static_cast<__nv_bfloat16*>(a->up);
+    q.gate_stride = a->gate_stride;
+    q.up_stride = a->up_stride;
     const int box = narrow_box(kNarrowProduct);
-    if (int rc = ffn_map(&p.a[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, box, "w_gate")) return rc;
-    if (int rc = ffn_map(&p.a[1], a->w_up, a->inner, a->hidden, a->w_up_stride, box, "w_up")) return rc;
-    if (int rc = ffn_map(&p.b[0], a->x, a->m, a->hidden, a->x_stride, p.columns, "x")) return rc;
-    if (int rc = launch_narrow(kNarrowProduct, p, false, call, st)) return rc;
+    if (int rc = ffn_map(&q.a[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, box, "w_gate")) return rc;
+    if (int rc = ffn_map(&q.a[1], a->w_up, a->inner, a->hidden, a->w_up_stride, box, "w_up")) return rc;
+    if (int rc = ffn_map(&q.b[0], a->x, a->m, a->hidden, a->x_stride, q.columns, "x")) return rc;
+    if (int rc = launch_narrow(kNarrowProduct, q, false, call, st)) return rc;
   } else {
     GemmParams p{};
     p.count = 1;
@@ -634,18 +646,13 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
     p.up_stride = a->up_stride;
     if (int rc = launch_gemm<false, false, kProduct>(p, 0, call, st)) return rc;
   }
-  if (few_tokens(a->m, a->out_dim, kb_out, kNarrowStore)) {
-    NarrowParams p{};
-    p.tokens = a->m;
-    p.columns = narrow_columns(a->m, a->out_dim);
-    p.features = a->out_dim;
-    p.kb = p.kb_first = kb_out;
-    p.out = static_cast<__nv_bfloat16*>(a->out);
-    p.out_stride = a->out_stride;
-    if (int rc = ffn_map(&p.a[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, narrow_box(kNarrowStore), "w_down"))
+  if (NarrowParams q{}; few_tokens(a->m, a->out_dim, kb_out, kNarrowStore, q)) {
+    q.out = static_cast<__nv_bfloat16*>(a->out);
+    q.out_stride = a->out_stride;
+    if (int rc = ffn_map(&q.a[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, narrow_box(kNarrowStore), "w_down"))
       return rc;
-    if (int rc = ffn_map(&p.b[0], h, a->m, a->inner, a->inner, p.columns, "workspace")) return rc;
-    return launch_narrow(kNarrowStore, p, true, call, st);
+    if (int rc = ffn_map(&q.b[0], h, a->m, a->inner, a->inner, q.columns, "workspace")) return rc;
+    return launch_narrow(kNarrowStore, q, true, call, st);
   }
   GemmParams p{};
   p.count = 1;
@@ -717,25 +724,20 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
   __nv_bfloat16* up = static_cast<__nv_bfloat16*>(const_cast<void*>(a->up));
   const int kb_dh = (int)div_up(a->out_dim, kFfnK), kb_inner = (int)div_up(a->inner, kFfnK);
   // dh = dout w_down, and what follows from it element by element
-  if (few_tokens(a->m, a->inner, kb_dh, kNarrowSlopes)) {
-    NarrowParams p{};
-    p.tokens = a->m;
-    p.columns = narrow_columns(a->m, a->inner);
-    p.features = a->inner;
-    p.kb = p.kb_first = kb_dh;
-    p.activation = a->activation;
-    p.out = a->dw_down != nullptr ? h : nullptr;
-    p.out_stride = p.dgate_stride = p.dup_stride = a->inner;
-    p.gate = gate;
-    p.up = up;
-    p.gate_stride = a->gate_stride;
-    p.up_stride = a->up_stride;
-    p.dgate = dgate;
-    p.dup = dup;
-    if (int rc = ffn_map(&p.a[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, narrow_box(kNarrowSlopes), "w_down"))
+  if (NarrowParams q{}; few_tokens(a->m, a->inner, kb_dh, kNarrowSlopes, q)) {
+    q.activation = a->activation;
+    q.out = a->dw_down != nullptr ? h : nullptr;
+    q.out_stride = q.dgate_stride = q.dup_stride = a->inner;
+    q.gate = gate;
+    q.up = up;
+    q.gate_stride = a->gate_stride;
+    q.up_stride = a->up_stride;
+    q.dgate = dgate;
+    q.dup = dup;
+    if (int rc = ffn_map(&q.a[0], a->w_down, a->out_dim, a->inner, a->w_down_stride, narrow_box(kNarrowSlopes), "w_down"))
       return rc;
-    if (int rc = ffn_map(&p.b[0], a->dout, a->m, a->out_dim, a->dout_stride, p.columns, "dout")) return rc;
-    if (int rc = launch_narrow(kNarrowSlopes, p, false, call, st)) return rc;
+    if (int rc = ffn_map(&q.b[0], a->dout, a->m, a->out_dim, a->dout_stride, q.columns, "dout")) return rc;
+    if (int rc = launch_narrow(kNarrowSlopes, q, false, call, st)) return rc;
   } else {
     GemmParams p{};
     p.count = 1;
@@ -757,21 +759,16 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     p.dgate_stride = p.dup_stride = a->inner;
     if (int rc = launch_gemm<false, true, kSlopes>(p, 2, call, st)) return rc;
   }
-  if (a->dx != nullptr && few_tokens(a->m, a->hidden, 2 * kb_inner, kNarrowStoreMN)) {
-    NarrowParams p{};
-    p.tokens = a->m;
-    p.columns = narrow_columns(a->m, a->hidden);
-    p.features = a->hidden;
-    p.kb = 2 * kb_inner;
-    p.kb_first = kb_inner;
-    p.out = static_cast<__nv_bfloat16*>(a->dx);
-    p.out_stride = a->dx_stride;
+  if (NarrowParams q{}; a->dx != nullptr && few_tokens(a->m, a->hidden, 2 * kb_inner, kNarrowStoreMN, q)) {
+    q.kb_first = kb_inner;
+    q.out = static_cast<__nv_bfloat16*>(a->dx);
+    q.out_stride = a->dx_stride;
     const int box = narrow_box(kNarrowStoreMN);
-    if (int rc = ffn_map(&p.a[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, box, "w_gate")) return rc;
-    if (int rc = ffn_map(&p.a[1], a->w_up, a->inner, a->hidden, a->w_up_stride, box, "w_up")) return rc;
-    if (int rc = ffn_map(&p.b[0], dgate, a->m, a->inner, a->inner, p.columns, "workspace")) return rc;
-    if (int rc = ffn_map(&p.b[1], dup, a->m, a->inner, a->inner, p.columns, "workspace")) return rc;
-    if (int rc = launch_narrow(kNarrowStoreMN, p, true, call, st)) return rc;
+    if (int rc = ffn_map(&q.a[0], a->w_gate, a->inner, a->hidden, a->w_gate_stride, box, "w_gate")) return rc;
+    if (int rc = ffn_map(&q.a[1], a->w_up, a->inner, a->hidden, a->w_up_stride, box, "w_up")) return rc;
+    if (int rc = ffn_map(&q.b[0], dgate, a->m, a->inner, a->inner, q.columns, "workspace")) return rc;
+    if (int rc = ffn_map(&q.b[1], dup, a->m, a->inner, a->inner, q.columns, "workspace")) return rc;
+    if (int rc = launch_narrow(kNarrowStoreMN, q, true, call, st)) return rc;
   } else if (a->dx != nullptr) {
     GemmParams p{};
     p.count = 1;
