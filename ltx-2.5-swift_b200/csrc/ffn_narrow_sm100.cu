@@ -340,10 +340,11 @@ int launch(NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
 // some of the 296 places empty.
 constexpr int kPlaces[kNMaxCluster + 1] = {0, 296, 296, 270, 264, 260, 264, 210, 240};
 
-// What a cut takes, in microseconds: 5.5 a call's share and 3 a round of CTAs; an SM brings in 1 KB of a K slice per
-// 10 ns, and 1 KB of another CTA's sums per 28 ns, for the one or two CTAs that it holds; and all weights come in at
-// 6.4 TB/s.  Fitted to 2700 cuts of 128 products (96 to 1024 tokens, 1024 to 16384 features): the cut that it finds
-// fastest is 0.8 us slower than the fastest one measured, on average.
+// What a cut takes, in microseconds: 2.5 a product and 3 a round of CTAs; an SM brings in 1 KB of a K slice per 10
+// ns, and 1 KB of another CTA's sums per 28 ns, for the one or two CTAs that it holds; and all weights come in at 6.4
+// TB/s, which takes the loads of 256 CTAs in flight (19 tokens at 2048 x 8192 with 128, 192 and 256 CTAs for the first
+// product: 32.3, 29.1 and 28.5 us for both).  Fitted to 2700 cuts of 128 products (96 to 1024 tokens, 1024 to 16384
+// features): the cut that it finds fastest is 0.8 us slower than the fastest one measured, on average.
 double cut_us(int parts, int tokens, int features, int kb, int columns, int cluster) {
   const int64_t ctas = div_up(features, kNRows) * div_up(tokens, columns) * cluster;
   const int64_t rounds = ctas / kPlaces[cluster], rest = ctas - rounds * kPlaces[cluster];
@@ -352,7 +353,8 @@ double cut_us(int parts, int tokens, int features, int kb, int columns, int clus
                      (cluster > 1 && columns * parts > 208 ? 1.5 : 0.0);  // the exchange in two pieces
   double us = 2.5 + rounds * (3.0 + 2 * cta);
   if (rest > 0) us += 3.0 + cta * (rest > 148 ? 2.0 : 1.0 + rest / 148.0);
-  return std::max(us, 5.5 + 2e-5 * features * parts * kb);
+  const double idle = std::max(0.0, (256.0 - ctas) / 128);
+  return std::max(us, 5.5 + 2e-5 * features * parts * kb * (1 + 0.28 * idle * idle));
 }
 
 // The fastest cut: token tiles as few as fit (128 columns each) or up to three more, 1 to 8 CTAs to a tile with a
