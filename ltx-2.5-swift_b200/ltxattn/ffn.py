@@ -68,6 +68,19 @@ def _out_rows(name: str, t: torch.Tensor) -> torch.Tensor:
     return rows
 
 
+def _gradient(name: str, t: Optional[torch.Tensor], of: Optional[torch.Tensor], like: torch.Tensor, shape, rows: int,
+              cols: int, device: int):
+    """The caller's output, or a new one, and its (address, row stride)."""
+    if t is None:
+        if of is not None and of.shape == shape and of.is_contiguous() and of.dtype == torch.bfloat16 and \
+                of.get_device() == device:
+            t = torch.empty_like(of)
+        else:
+            t = _output(name, None, shape, like)
+        return t, (t.data_ptr(), cols)
+    return t, _matrix(name, _out_rows(name, _output(name, t, shape, like)), rows, cols, device)
+
+
 def _first_dim(name: str, w: torch.Tensor) -> int:
     if not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise Failure.shape(name, getattr(w, "shape", ()), "a matrix")
@@ -131,40 +144,41 @@ def gated_ffn_backward(x: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: to
     if dout.dim() < 1:
         raise Failure.shape("dout", dout.shape, "[..., out]")
     device = dout.get_device()
-    if not isinstance(w_gate, torch.Tensor) or w_gate.dim() != 2:
-        raise Failure.shape("w_gate", getattr(w_gate, "shape", ()), "a matrix")
-    inner, hidden = w_gate.shape
+    inner = _first_dim("w_gate", w_gate)
+    hidden = w_gate.shape[1]
     if x is None and need_dw:
         raise Failure("missing", "x is needed for the gradients of w_gate and w_up")
     lead = dout.shape[:-1]
-    for name, t, cols in (("x", x, hidden), ("gate", gate, inner), ("up", up, inner)):
-        if t is None and name == "x":
-            continue
-        _check_cuda(name, t)
-        if tuple(t.shape) != tuple(lead) + (cols,):
-            raise Failure.shape(name, t.shape, str(list(lead) + [cols]))
+    if len(lead) != 1:  # a matrix is checked as such below
+        for name, t, cols in (("x", x, hidden), ("gate", gate, inner), ("up", up, inner)):
+            if t is not None or name != "x":
+                _check_cuda(name, t)
+                if t.shape != lead + (cols,):
+                    raise Failure.shape(name, t.shape, str(list(lead) + [cols]))
     with _on(device, stream) as st:
-        d2 = _rows("dout", dout)
+        if len(lead) == 1:
+            d2, x2, gate2, up2 = dout, x, gate, up
+        else:
+            d2, gate2, up2 = _rows("dout", dout), _rows("gate", gate), _rows("up", up)
+            x2 = None if x is None else _rows("x", x)
         m, out_dim = d2.shape
-        x2, gate2, up2 = (None if t is None else _rows(name, t) for name, t in (("x", x), ("gate", gate), ("up", up)))
-        if need_dx:
-            dx = _output("dx", dx, tuple(lead) + (hidden,), dout)
-        if need_dw:
-            dw_gate = _output("dw_gate", dw_gate, (inner, hidden), dout)
-            dw_up = _output("dw_up", dw_up, (inner, hidden), dout)
-            dw_down = _output("dw_down", dw_down, (out_dim, inner), dout)
         nothing = (0, 0)
-        args = (_lib.BF16, act, m, hidden, inner, out_dim,
-                *(nothing if x2 is None else _matrix("x", x2, m, hidden, device)),
+        to = [nothing] * 4
+        if need_dx:
+            dx, to[0] = _gradient("dx", dx, x, dout, lead + (hidden,), m, hidden, device)
+        if need_dw:
+            dw_gate, to[1] = _gradient("dw_gate", dw_gate, w_gate, dout, (inner, hidden), inner, hidden, device)
+            dw_up, to[2] = _gradient("dw_up", dw_up, w_up, dout, (inner, hidden), inner, hidden, device)
+            dw_down, to[3] = _gradient("dw_down", dw_down, w_down, dout, (out_dim, inner), out_dim, inner, device)
+        ws = _planes(3, m, inner, dout)
+        rc = _lib.load().ltxattn_gated_ffn_bwd(
+            _lib.GATED_FFN_BWD_ARGS.pack(
+                _lib.BF16, act, m, hidden, inner, out_dim,
+                *(nothing if x is None else _matrix("x", x2, m, hidden, device)),
                 *_matrix("w_gate", w_gate, inner, hidden, device), *_matrix("w_up", w_up, inner, hidden, device),
                 *_matrix("w_down", w_down, out_dim, inner, device), *_matrix("gate", gate2, m, inner, device),
-                *_matrix("up", up2, m, inner, device), *_matrix("dout", d2, m, out_dim, device),
-                *(_matrix("dx", _out_rows("dx", dx), m, hidden, device) if need_dx else nothing),
-                *(_matrix("dw_gate", dw_gate, inner, hidden, device) if need_dw else nothing),
-                *(_matrix("dw_up", dw_up, inner, hidden, device) if need_dw else nothing),
-                *(_matrix("dw_down", dw_down, out_dim, inner, device) if need_dw else nothing))
-        ws = _planes(3, m, inner, dout)
-        rc = _lib.load().ltxattn_gated_ffn_bwd(_lib.GATED_FFN_BWD_ARGS.pack(*args, ws.data_ptr(), ws.numel()), st)
+                *_matrix("up", up2, m, inner, device), *_matrix("dout", d2, m, out_dim, device), *to[0], *to[1],
+                *to[2], *to[3], ws.data_ptr(), ws.numel()), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
     return (dx if need_dx else None,) + ((dw_gate, dw_up, dw_down) if need_dw else (None, None, None))
