@@ -51,6 +51,7 @@ struct RotaryEmbedParams {
   int slots;         // slots of a token: turned ones, then copied ones
   int turn_slots;    // pairs / kP
   int slot_lanes, head_lanes, token_lanes;  // a CTA's threads
+  int head_groups;
   const double* freq;
   const void* positions;  // or null: token t stands at t
   int pos64;
@@ -135,29 +136,39 @@ struct Slot {
   int at, apart;  // the first run in a head, and from it to the second
   float c[kP], s[kP];
 
-  // through the heads h, h + step, ... of a view's token
+  // through the heads h, h + step, ... of a view's token; short runs take several heads at once, to have as many
+  // bytes on their way as a long one
   __device__ __forceinline__ void walk(const RView& v, int64_t b, int64_t t, int h, int step) const {
     using R = Run<T, kRun>;
+    constexpr int kAtOnce = sizeof(R) >= 16 ? 1 : sizeof(R) == 8 ? 2 : 4;
     const T* x = static_cast<const T*>(v.x) + b * v.x_sb + t * v.x_st + h * v.x_sh + at;
     T* y = static_cast<T*>(v.y) + b * v.y_sb + t * v.y_st + h * v.y_sh + at;
     const int64_t dx = step * v.x_sh, dy = step * v.y_sh;
 #pragma unroll 1
-    for (; h < v.heads; h += step, x += dx, y += dy) {
-      R r0 = load_run<R>(x);
-      if (turned) {
-        R r1;
-        if (kTwoRuns) r1 = load_run<R>(x + apart);
+    for (; h < v.heads; h += kAtOnce * step, x += kAtOnce * dx, y += kAtOnce * dy) {
+      R r0[kAtOnce], r1[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < kP; ++e) {
-          T& ea = kTwoRuns ? r0.e[e] : r0.e[(2 * e) % kRun];
-          T& eb = kTwoRuns ? r1.e[e] : r0.e[(2 * e + 1) % kRun];
-          const float fa = to_f(ea), fb = to_f(eb);
-          from_f(ea, fmaf(fa, c[e], -(fb * s[e])));
-          from_f(eb, fmaf(fb, c[e], fa * s[e]));
-        }
-        if (kTwoRuns) store_run(y + apart, r1);
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (u > 0 && h + u * step >= v.heads) break;
+        r0[u] = load_run<R>(x + u * dx);
+        if (kTwoRuns && turned) r1[u] = load_run<R>(x + u * dx + apart);
       }
-      store_run(y, r0);
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (u > 0 && h + u * step >= v.heads) break;
+        if (turned) {
+#pragma unroll
+          for (int e = 0; e < kP; ++e) {
+            T& ea = kTwoRuns ? r0[u].e[e] : r0[u].e[(2 * e) % kRun];
+            T& eb = kTwoRuns ? r1[u].e[e] : r0[u].e[(2 * e + 1) % kRun];
+            const float fa = to_f(ea), fb = to_f(eb);
+            from_f(ea, fmaf(fa, c[e], -(fb * s[e])));
+            from_f(eb, fmaf(fb, c[e], fa * s[e]));
+          }
+          if (kTwoRuns) store_run(y + u * dy + apart, r1[u]);
+        }
+        store_run(y + u * dy, r0[u]);
+      }
     }
   }
 };
@@ -165,7 +176,8 @@ struct Slot {
 // A CTA takes token_lanes tokens (one, unless its heads are few) with all their
 // heads.  Its threads first make the tokens' cos and sin, into shared memory;
 // then thread (slot, head lane, token) keeps its slot's in registers and walks
-// over every head_lanes-th head of q and of k.  The heads of a token lie side by
+// over every head_lanes-th head of q and of k (few tokens: the heads are shared
+// by gridDim.y CTAs, each making the cos and sin again).  The heads of a token lie side by
 // side in a projection's output, so a CTA streams whole rows of it.  Many small
 // CTAs keep the memory busy better than more runs per thread: 128 threads at 48
 // registers take 150 us for 29760 tokens x 64 heads x 128 in bf16 (6.5 TB/s, 0.99
@@ -190,7 +202,8 @@ __global__ void __launch_bounds__(kRThreads, 5) rotary_embed_kernel(const __grid
   }
   __syncthreads();
   using S = Slot<T, kP, kInterleaved>;
-  const int rest = threadIdx.x / p.slot_lanes, r = rest / p.head_lanes, h0 = rest - r * p.head_lanes;
+  const int rest = threadIdx.x / p.slot_lanes, r = rest / p.head_lanes;
+  const int h0 = blockIdx.y * p.head_lanes + rest - r * p.head_lanes, step = gridDim.y * p.head_lanes;
   if (r >= n_rows) return;
   const int64_t b = (row0 + r) / p.T, t = (row0 + r) - b * p.T;
   for (int slot = threadIdx.x % p.slot_lanes; slot < p.slots; slot += p.slot_lanes) {
@@ -204,8 +217,8 @@ __global__ void __launch_bounds__(kRThreads, 5) rotary_embed_kernel(const __grid
       w.c[e] = cs.x;
       w.s[e] = cs.y;
     }
-    w.walk(p.v[0], b, t, h0, p.head_lanes);
-    w.walk(p.v[1], b, t, h0, p.head_lanes);
+    w.walk(p.v[0], b, t, h0, step);
+    w.walk(p.v[1], b, t, h0, step);
   }
 }
 
@@ -220,7 +233,7 @@ int fail_rotary(int status, const char* fmt, ...) {
 
 template <typename T, int kP>
 void launch(const RotaryEmbedParams& p, bool interleaved, cudaStream_t st) {
-  const unsigned grid = (unsigned)((p.rows + (int64_t)p.token_lanes - 1) / p.token_lanes);
+  const dim3 grid((unsigned)((p.rows + (int64_t)p.token_lanes - 1) / p.token_lanes), (unsigned)p.head_groups);
   const int threads = p.slot_lanes * p.head_lanes * p.token_lanes;
   const size_t smem = sizeof(float2) * p.token_lanes * p.pairs;
   if (interleaved)
@@ -378,6 +391,9 @@ int ltxattn_rotary_embed(const ltxattn_rotary_embed_args* a, void* stream) {
   p.inverse = a->inverse != 0;
   p.slot_lanes = std::min(p.slots, kRThreads);
   p.head_lanes = std::max(1, std::min((int)std::max(H, Hk), kTargetThreads / p.slot_lanes));
+  // few tokens: as many CTAs to a token as fill the GPU, at a head to a thread at least
+  const int64_t threads = std::min<int64_t>(int64_t(p.rows) * p.slot_lanes * p.head_lanes, 148 * 1024);
+  p.head_groups = (int)std::min<int64_t>({148 * 1024 / threads, (std::max(H, Hk) + p.head_lanes - 1) / p.head_lanes, 65535});
   p.token_lanes = std::max(1, kTargetThreads / (p.slot_lanes * p.head_lanes));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (bf16) {
