@@ -63,6 +63,9 @@ def row(B, T, offset=0):
     (3, 7, 2, 1, 37, 6),         # an odd head size: single elements
     (1, 1030, 40, 1, 256, 250),
     (1, 300, 64, 64, 128, 128),
+    (2, 20000, 2, 1, 64, 64),    # many tokens of few heads: a thread through all heads of a token
+    (1, 30011, 3, 2, 40, 24),
+    (3, 9001, 1, 1, 37, 6),
 ])
 def test_matches_the_rotation(layout, dtype, B, T, H, Hk, D, rot):
     q, k = heads(1, B, T, H, D, dtype), heads(2, B, T, Hk, D, dtype)
