@@ -67,12 +67,12 @@ __device__ __forceinline__ void slopes(float g, float u, float dh, float& dg, fl
   h = a * u;
 }
 
-// 8 consecutive bf16 of a row (16-byte aligned).
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                                            pack_bf16x2(v[6], v[7]));
+// 8 of v, from `at` on, as bf16.
+template <int kN>
+__device__ __forceinline__ uint4 pack8(const float (&v)[kN], int at = 0) {
+  return make_uint4(pack_bf16x2(v[at], v[at + 1]), pack_bf16x2(v[at + 2], v[at + 3]),
+                    pack_bf16x2(v[at + 4], v[at + 5]), pack_bf16x2(v[at + 6], v[at + 7]));
 }
-
 __device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -117,8 +117,10 @@ __device__ __forceinline__ uint32_t peer_address(uint32_t local, uint32_t rank) 
 // Records the message and gives the status back.
 int fail_ffn(int status, const char* fmt, ...);
 
-// bf16 [rows, cols], `stride` elements between rows; boxes of 64 columns (one swizzle row) and box_rows rows.
-int ffn_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t stride, int box_rows, const char* name);
+// bf16 [rows, cols], `stride` elements between rows; boxes of box_cols columns (64 or 32: one row of the 128- or
+// 64-byte swizzle) and box_rows rows.
+int ffn_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t stride, int box_rows, const char* name,
+            int box_cols = 64);
 
 constexpr int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

@@ -59,32 +59,34 @@ constexpr int kGEpilogueWarps = 8;
 
 enum Epilogue { kProduct, kStore, kSlopes };
 
-// The epilogue's warps pass their 32 rows x 32 columns through shared memory, so that they are written (and the
-// kept gate and up read) as whole 64-byte pieces of rows: a thread finds a row in TMEM, and storing rows from
-// there takes a line of memory per thread and access.  Rows are padded to 80 (bf16) or 144 bytes (fp32), which
-// spreads eight of them over all banks.
-constexpr uint32_t kRowBf16 = 80, kRowF32 = 144;
+// The epilogue's warps pass their 32 rows through shared memory, 32 columns in bf16 at a time, and TMA carries those
+// pieces out (and the kept gate and up in): a thread finds a row in TMEM, and accesses of one row per thread take a
+// line of memory each.  A piece is 32 rows of 64 bytes in the 64-byte swizzle, which lets eight rows' threads touch all
+// banks.
+constexpr uint32_t kPiece = 32 * 64;
 
 template <int kEpilogue>
-struct GemmSmem {
-  static constexpr int kStages = kEpilogue == kSlopes ? 5 : 6;
-  static constexpr uint32_t kRow = kEpilogue == kSlopes ? kRowF32 : kRowBf16;
-  static constexpr uint32_t kOffStaging = kStages * kGStage;
-  // full[kStages] (the first CTA's counts for both), empty[kStages], acc_full[2], acc_empty[2] (the first CTA's)
-  static constexpr uint32_t kOffBar = kOffStaging + 8 * 32 * kRow;
-  static constexpr uint32_t kOffCtl = kOffBar + (2 * kStages + 4) * 8;  // TMEM slot, abort flag
-  static constexpr uint32_t kBytes = kOffCtl + 16 + 1024;               // + alignment slack
+struct GemmShape {
+  // Pieces per warp.  Products go out through two in turn.  The gradient's epilogue has two of gate and up in turn, in
+  // which dgate and dup take their place, and one of h.
+  static constexpr int kPieces = kEpilogue == kSlopes ? 5 : 2;
+  static constexpr int kStages = kEpilogue == kSlopes ? 4 : 5;
+  static constexpr uint32_t kOffPieces = kStages * kGStage;
+  // full[kStages] (the first CTA's counts for both), empty[kStages], acc_full[2], acc_empty[2] (the first CTA's), and
+  // two for the gate and up of each warp
+  static constexpr uint32_t kOffBar = kOffPieces + kGEpilogueWarps * kPieces * kPiece;
+  static constexpr uint32_t kOffCtl = kOffBar + (2 * kStages + 4 + 2 * kGEpilogueWarps) * 8;  // TMEM slot, abort flag
+  static constexpr uint32_t kBytes = kOffCtl + 16 + 1024;                                     // + alignment slack
   static_assert(kBytes <= kMaxDynamicSmem, "shared memory of a CTA");
 };
 
 // One output of a launch (a launch of the weight gradients has up to three).
 struct Gemm {
   CUtensorMap a[2], b[2];  // K slices beyond kb_first come from the second pair
+  CUtensorMap out;         // in pieces of 32 x 32
   int M, N;                // rows and accumulator columns that exist (kProduct: columns of h)
   int kb, kb_first;        // 64-wide K slices in all, and those of the first pair
   int tiles_m, tiles_n;
-  __nv_bfloat16* out;
-  int64_t out_stride;
 };
 
 struct GemmParams {
@@ -92,9 +94,10 @@ struct GemmParams {
   int first_tile[4];  // tiles of g[i]: [first_tile[i], first_tile[i + 1])
   int count;
   int activation;
-  // kProduct: gate and up to be kept (or null).  kSlopes: the kept ones, and dgate and dup
-  __nv_bfloat16 *gate, *up, *dgate, *dup;
-  int64_t gate_stride, up_stride, dgate_stride, dup_stride;
+  // kProduct: gate and up to be kept (where `keep`).  kSlopes: the kept ones, and dgate and dup; h goes to out where
+  // `keep`
+  CUtensorMap gate, up, dgate, dup;
+  int keep;
   int* err;
 };
 
@@ -125,20 +128,23 @@ __device__ __forceinline__ void pair_tmem_alloc(uint32_t* slot, uint32_t columns
 __device__ __forceinline__ void pair_tmem_free(uint32_t tmem, uint32_t columns) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
+// Issued by the whole warp with the same operands, one elected lane doing it: they then stay in uniform registers, and
+// the issue keeps up beside the epilogue warps that share the scheduler.
 __device__ __forceinline__ void pair_mma(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
                                          uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\t"
       "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}\n" ::"r"(d),
+      "setp.ne.b32 p, %6, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}\n" ::"r"(d),
       "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Arrives at `bar` of both CTAs once every MMA issued so far is done.
+// Arrives at `bar` of both CTAs once every MMA issued so far is done (the whole warp; the same lane is elected).
 __device__ __forceinline__ void pair_commit(uint64_t* bar) {
   asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}\n" ::"r"(
           smem_u32(bar)),
       "h"(static_cast<uint16_t>(3))
       : "memory");
@@ -155,38 +161,58 @@ __device__ __forceinline__ void cluster_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// 32 rows (one per lane) x 32 columns of the warp to bf16 rows of global memory, from `row0` and `col` on; what is
-// outside M x N is left out.
-__device__ __forceinline__ void flush(uint8_t* staging, int lane, const float (&v)[32], __nv_bfloat16* out,
-                                      int64_t stride, int64_t row0, int col, int M, int N) {
-  uint4* mine = reinterpret_cast<uint4*>(staging + lane * kRowBf16);
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    mine[q] = make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
-                         pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
-  __syncwarp();
-  const int piece = lane & 3;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = (lane >> 2) + 8 * i;
-    const uint4 w = *reinterpret_cast<const uint4*>(staging + r * kRowBf16 + piece * 16);
-    if (row0 + r < M && col + 8 * piece < N)
-      *reinterpret_cast<uint4*>(out + (row0 + r) * stride + col + 8 * piece) = w;
-  }
-  __syncwarp();
+__device__ __forceinline__ void piece_store(const CUtensorMap* map, uint32_t piece, int col, int row) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(piece), "r"(col), "r"(row)
+               : "memory");
 }
+// Waits until at most kPending of this thread's groups of stores still read their pieces.
+template <int kPending>
+__device__ __forceinline__ void piece_wait() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPending) : "memory");
+}
+// 8 columns (16 bytes) of a row in a piece.
+__device__ __forceinline__ uint4* in_piece(uint8_t* piece, int row, int q) {
+  return reinterpret_cast<uint4*>(piece + row * 64 + ((q ^ ((row >> 1) & 3)) << 4));
+}
+
+// The two pieces that a warp's products go out through, in turn.
+struct Outgoing {
+  uint8_t* pieces;
+  int lane;
+  int next = 0;
+
+  // 32 rows (one per lane) x 32 columns; what is outside the tensor is left out
+  __device__ __forceinline__ void send(const CUtensorMap* map, const float (&v)[32], int col, int row) {
+    uint8_t* piece = pieces + next * kPiece;
+    next ^= 1;
+    if (lane == 0) piece_wait<1>();  // the one before the last has been read
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *in_piece(piece, lane, q) = pack8(v, 8 * q);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      piece_store(map, smem_u32(piece), col, row);
+      bulk_commit();
+    }
+  }
+};
 
 template <bool kAMN, bool kBMN, int kEpilogue>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
     gemm_kernel(const __grid_constant__ GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = align1024(smem_raw);
-  using S = GemmSmem<kEpilogue>;
+  using S = GemmShape<kEpilogue>;
   constexpr int kGStages = S::kStages;
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + S::kOffBar);
   uint64_t* empty = full + kGStages;
   uint64_t* acc_full = empty + kGStages;
   uint64_t* acc_empty = acc_full + 2;
+  uint64_t* kept_full = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + S::kOffCtl);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + S::kOffCtl + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -200,6 +226,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
       mbar_init(acc_full + i, 1);
       mbar_init(acc_empty + i, 2 * kGEpilogueWarps);
     }
+    for (int i = 0; i < 2 * kGEpilogueWarps; ++i) mbar_init(kept_full + i, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -258,7 +285,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
     // never leave the CTA with a bulk copy still writing its shared memory: a stage is empty again once it was
     // full and has been read
     for (int i = it < kGStages ? 0 : it - kGStages; i < it; ++i) drain_wait(empty + i % kGStages, (i / kGStages) & 1);
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0) {
     constexpr uint32_t idesc = idesc_bf16_f32(kGPairM, kGN, kAMN, kBMN);
     const SDesc a0 = sdesc_split(smem_u32(sm), kAMN ? kChunk : 16, 1024);
     const SDesc b0 = sdesc_split(smem_u32(sm) + kGA, kBMN ? kChunk : 16, 1024);
@@ -271,12 +298,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
       locate(p, tile, which, m0, tn);
       const int kb_n = p.g[which].kb;
       const int buf = n & 1;
-      if (n >= 2 && !mbar_wait(acc_empty + buf, ((n >> 1) - 1) & 1, abort_flag, p.err, 62)) break;
+      if (n >= 2 && !warp_wait(acc_empty + buf, ((n >> 1) - 1) & 1, abort_flag, p.err, 62)) break;
       tc_fence_after();
       const uint32_t d = tmem + buf * kGN;
       for (int kb = 0; kb < kb_n; ++kb, ++it) {
         const int st = it % kGStages, u = it / kGStages;
-        if (!mbar_wait(full + st, u & 1, abort_flag, p.err, 63)) {
+        if (!warp_wait(full + st, u & 1, abort_flag, p.err, 63)) {
           ok = false;
           break;
         }
@@ -294,33 +321,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
   } else if (warp >= 4) {
     const int quadrant = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lane_off = static_cast<uint32_t>(quadrant * 32) << 16;
-    uint8_t* staging = sm + S::kOffStaging + (warp - 4) * 32 * S::kRow;
-    int n = 0;
+    uint8_t* pieces = sm + S::kOffPieces + (warp - 4) * S::kPieces * kPiece;
+    Outgoing outgoing{pieces, lane};
+    uint64_t* kept = kept_full + 2 * (warp - 4);
+    int n = 0, turn = 0;  // turn: uses of the gate and up pieces
     for (int tile = first; tile < tiles; tile += step, ++n) {
       int which, m0, tn;
       locate(p, tile, which, m0, tn);
       const Gemm& g = p.g[which];
       const int buf = n & 1;
-      const int64_t row0 = m0 + rank * kGM + quadrant * 32;
-      // 4 lanes to a row of 32 columns, in the order that flush() writes
-      const int piece = lane & 3;
-      uint4 gw[4], uw[4];  // kSlopes: the kept gate and up of the next 32 columns
-      auto fetch = [&](int c) {
-        const int col = tn * kGN + c + 8 * piece;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t row = row0 + (lane >> 2) + 8 * i;
-          gw[i] = uw[i] = make_uint4(0, 0, 0, 0);
-          if (row < g.M && col < g.N) {
-            gw[i] = *reinterpret_cast<const uint4*>(p.gate + row * p.gate_stride + col);
-            uw[i] = *reinterpret_cast<const uint4*>(p.up + row * p.up_stride + col);
-          }
+      const int row0 = m0 + rank * kGM + quadrant * 32;
+      // kSlopes: the columns of gate and up for this warp's next turn, on their way
+      auto fetch = [&](int c, int t) {
+        const int col = tn * kGN + half * 128 + c;
+        if (lane == 0 && c < 128 && col < g.N && row0 < g.M) {
+          mbar_arrive_expect_tx(kept + (t & 1), 2 * kPiece);
+          tma_load_2d(&p.gate, kept + (t & 1), pieces + (t & 1) * 2 * kPiece, col, row0);
+          tma_load_2d(&p.up, kept + (t & 1), pieces + (t & 1) * 2 * kPiece + kPiece, col, row0);
         }
       };
-      if (kEpilogue == kSlopes) fetch(half * 128);
-      if (!warp_wait(acc_full + buf, (n >> 1) & 1, abort_flag, p.err, 64)) break;
+      if (kEpilogue == kSlopes) {
+        if (lane == 0) piece_wait<0>();
+        fetch(0, turn);
+      }
+      if (!warp_wait(acc_full + buf, (n >> 1) & 1, abort_flag, p.err, 64)) {
+        // never leave the CTA with a copy still writing its shared memory
+        if (kEpilogue == kSlopes && lane == 0 && row0 < g.M && tn * kGN + half * 128 < g.N)
+          drain_wait(kept + (turn & 1), (turn >> 1) & 1);
+        break;
+      }
       tc_fence_after();
       const uint32_t d = tmem + buf * kGN + lane_off;
+      // The accumulator is free for the tile after the next once this warp has its last columns in registers.
+      bool released = false;
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) cluster_arrive(peer_address(smem_u32(acc_empty + buf), 0));
+        released = true;
+      };
       if (row0 >= g.M) {
         // nothing of this warp's exists
       } else if (kEpilogue == kProduct) {
@@ -334,14 +373,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
           tmem_ld32(d + c, rg);
           tmem_ld32(d + kGHalfN + c, ru);
           tmem_wait_ld();
+          if (c + 32 == half * 64 + 64) release();
           float v[32];
-          if (p.gate != nullptr) {
+          if (p.keep) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(rg[e]);
-            flush(staging, lane, v, p.gate, p.gate_stride, row0, col, g.M, g.N);
+            outgoing.send(&p.gate, v, col, row0);
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(ru[e]);
-            flush(staging, lane, v, p.up, p.up_stride, row0, col, g.M, g.N);
+            outgoing.send(&p.up, v, col, row0);
           }
           with_activation(p.activation, [&](auto act) {
             float unused;
@@ -349,7 +389,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
             for (int e = 0; e < 32; ++e)
               v[e] = activate<decltype(act)::value, false>(__uint_as_float(rg[e]), unused) * __uint_as_float(ru[e]);
           });
-          flush(staging, lane, v, g.out, g.out_stride, row0, col, g.M, g.N);
+          outgoing.send(&g.out, v, col, row0);
         }
       } else if (kEpilogue == kStore) {
 #pragma unroll 1
@@ -360,55 +400,56 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
           uint32_t r[32];
           tmem_ld32(d + c, r);
           tmem_wait_ld();
+          if (c + 32 == half * 128 + 128) release();
           float v[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
-          flush(staging, lane, v, g.out, g.out_stride, row0, col, g.M, g.N);
+          outgoing.send(&g.out, v, col, row0);
         }
       } else {
 #pragma unroll 1
-        for (int c = half * 128; c < half * 128 + 128; c += 32) {
-          const int col = tn * kGN + c;
+        for (int c = 0; c < 128; c += 32, ++turn) {
+          const int col = tn * kGN + half * 128 + c;
           if (col >= g.N) break;  // warp-uniform
+          if (lane == 0) piece_wait<0>();  // the turn before has been read, its pieces are free
+          fetch(c + 32, turn + 1);
           __syncwarp();
           uint32_t r[32];
-          tmem_ld32(d + c, r);
+          tmem_ld32(d + half * 128 + c, r);
+          const bool here = warp_wait(kept + (turn & 1), (turn >> 1) & 1, abort_flag, p.err, 68);
           tmem_wait_ld();
-          uint4 now_g[4], now_u[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) now_g[i] = gw[i], now_u[i] = uw[i];
-          if (c + 32 < half * 128 + 128) fetch(c + 32);
-          uint4* mine = reinterpret_cast<uint4*>(staging + lane * kRowF32);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) mine[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
-          __syncwarp();
+          if (c + 32 == 128) release();
+          if (!here) continue;
+          uint8_t* gp = pieces + (turn & 1) * 2 * kPiece;
+          uint8_t* hp = pieces + 4 * kPiece;
           with_activation(p.activation, [&](auto act) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int rr = (lane >> 2) + 8 * i;
-              const float4* src = reinterpret_cast<const float4*>(staging + rr * kRowF32 + piece * 32);
-              const float4 lo = src[0], hi = src[1];
-              const float dh[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            for (int q = 0; q < 4; ++q) {
+              uint4 *gq = in_piece(gp, lane, q), *uq = in_piece(gp + kPiece, lane, q);
               float gv[8], uv[8], dgv[8], duv[8], hv[8];
-              unpack8(now_g[i], gv);
-              unpack8(now_u[i], uv);
+              unpack8(*gq, gv);
+              unpack8(*uq, uv);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) slopes<decltype(act)::value>(gv[e], uv[e], dh[e], dgv[e], duv[e], hv[e]);
-              const int64_t row = row0 + rr;
-              if (row < g.M && col + 8 * piece < g.N) {
-                store8(p.dgate + row * p.dgate_stride + col + 8 * piece, dgv);
-                store8(p.dup + row * p.dup_stride + col + 8 * piece, duv);
-                if (g.out != nullptr)  // h is wanted for dw_down alone
-                  store8(g.out + row * g.out_stride + col + 8 * piece, hv);
-              }
+              for (int e = 0; e < 8; ++e)
+                slopes<decltype(act)::value>(gv[e], uv[e], __uint_as_float(r[8 * q + e]), dgv[e], duv[e], hv[e]);
+              *gq = pack8(dgv);
+              *uq = pack8(duv);
+              *in_piece(hp, lane, q) = pack8(hv);
             }
           });
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            piece_store(&p.dgate, smem_u32(gp), col, row0);
+            piece_store(&p.dup, smem_u32(gp + kPiece), col, row0);
+            if (p.keep) piece_store(&g.out, smem_u32(hp), col, row0);
+            bulk_commit();
+          }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) cluster_arrive(peer_address(smem_u32(acc_empty + buf), 0));
+      if (!released) release();
     }
+    if (lane == 0) piece_wait<0>();  // the CTA's shared memory must outlive the copies' reads
   }
   __syncwarp();
   tc_fence_before();
@@ -454,15 +495,16 @@ int fail_ffn(int status, const char* fmt, ...) {
 }
 
 int ffn_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t stride, int box_rows,
-            const char* name) {
+            const char* name, int box_cols) {
   EncodeTiledFn enc = encoder();
   if (!enc) return fail_ffn(LTXATTN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
-  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail_ffn(LTXATTN_ERR_ALIGN, "%s: cuTensorMapEncodeTiled rejected the view (CUresult %d)", name, (int)r);
@@ -470,6 +512,11 @@ int ffn_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t
 }
 
 namespace {
+
+// The pieces that an epilogue's warp stores and loads: boxes of 32 x 32.
+int piece_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t stride, const char* name) {
+  return ffn_map(m, ptr, rows, cols, stride, 32, name, 32);
+}
 
 // A bf16 matrix argument.
 struct Mat {
@@ -542,7 +589,7 @@ int launch_gemm(GemmParams& p, int slot, const char* call, cudaStream_t st) {
   p.err = device_error_word();
   if (!p.err) return fail_ffn(LTXATTN_ERR_CUDA, "no device error word");
   int sms = 0;
-  constexpr uint32_t smem = GemmSmem<kEpilogue>::kBytes;
+  constexpr uint32_t smem = GemmShape<kEpilogue>::kBytes;
   cudaError_t e = prepare_kernel(gemm_kernel<kAMN, kBMN, kEpilogue>, slot, smem, &sms);
   if (e == cudaSuccess)
     e = launch_pdl(gemm_kernel<kAMN, kBMN, kEpilogue>, 2 * (unsigned)std::min<int64_t>(tiles, sms / 2), kGThreads, smem,
@@ -638,12 +685,12 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
     g.M = a->m;
     g.N = a->inner;
     g.kb = g.kb_first = kb_in;
-    g.out = h;
-    g.out_stride = a->inner;
-    p.gate = static_cast<__nv_bfloat16*>(a->gate);
-    p.up = static_cast<__nv_bfloat16*>(a->up);
-    p.gate_stride = a->gate_stride;
-    p.up_stride = a->up_stride;
+    if (int rc = piece_map(&g.out, h, a->m, a->inner, a->inner, "workspace")) return rc;
+    p.keep = a->gate != nullptr;
+    if (p.keep) {
+      if (int rc = piece_map(&p.gate, a->gate, a->m, a->inner, a->gate_stride, "gate")) return rc;
+      if (int rc = piece_map(&p.up, a->up, a->m, a->inner, a->up_stride, "up")) return rc;
+    }
     if (int rc = launch_gemm<false, false, kProduct>(p, 0, call, st)) return rc;
   }
   if (NarrowParams q{}; few_tokens(a->m, a->out_dim, kb_out, kNarrowStore, q)) {
@@ -662,8 +709,7 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
   g.M = a->m;
   g.N = a->out_dim;
   g.kb = g.kb_first = kb_out;
-  g.out = static_cast<__nv_bfloat16*>(a->out);
-  g.out_stride = a->out_stride;
+  if (int rc = piece_map(&g.out, a->out, a->m, a->out_dim, a->out_stride, "out")) return rc;
   return launch_gemm<false, false, kStore>(p, 1, call, st);
 }
 
@@ -748,15 +794,13 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     g.M = a->m;
     g.N = a->inner;
     g.kb = g.kb_first = kb_dh;
-    g.out = a->dw_down != nullptr ? h : nullptr;
-    g.out_stride = a->inner;
-    p.gate = gate;
-    p.up = up;
-    p.gate_stride = a->gate_stride;
-    p.up_stride = a->up_stride;
-    p.dgate = dgate;
-    p.dup = dup;
-    p.dgate_stride = p.dup_stride = a->inner;
+    p.keep = a->dw_down != nullptr;
+    if (p.keep)
+      if (int rc = piece_map(&g.out, h, a->m, a->inner, a->inner, "workspace")) return rc;
+    if (int rc = piece_map(&p.gate, a->gate, a->m, a->inner, a->gate_stride, "gate")) return rc;
+    if (int rc = piece_map(&p.up, a->up, a->m, a->inner, a->up_stride, "up")) return rc;
+    if (int rc = piece_map(&p.dgate, dgate, a->m, a->inner, a->inner, "workspace")) return rc;
+    if (int rc = piece_map(&p.dup, dup, a->m, a->inner, a->inner, "workspace")) return rc;
     if (int rc = launch_gemm<false, true, kSlopes>(p, 2, call, st)) return rc;
   }
   if (NarrowParams q{}; a->dx != nullptr && few_tokens(a->m, a->hidden, 2 * kb_inner, kNarrowStoreMN, q)) {
@@ -781,13 +825,12 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     g.N = a->hidden;
     g.kb = 2 * kb_inner;
     g.kb_first = kb_inner;
-    g.out = static_cast<__nv_bfloat16*>(a->dx);
-    g.out_stride = a->dx_stride;
+    if (int rc = piece_map(&g.out, a->dx, a->m, a->hidden, a->dx_stride, "dx")) return rc;
     if (int rc = launch_gemm<false, true, kStore>(p, 3, call, st)) return rc;
   }
   GemmParams p{};
   auto weight = [&](const void* at, int64_t at_stride, int rows, const void* b, int64_t b_stride, int cols, void* out,
-                    int64_t out_stride, const char* an, const char* bn) {
+                    int64_t out_stride, const char* an, const char* bn, const char* on) {
     if (out == nullptr) return (int)LTXATTN_OK;
     Gemm& g = p.g[p.count++];
     if (int rc = ffn_map(&g.a[0], at, a->m, rows, at_stride, kGK, an)) return rc;
@@ -795,17 +838,16 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     g.M = rows;
     g.N = cols;
     g.kb = g.kb_first = (int)div_up(a->m, kGK);
-    g.out = static_cast<__nv_bfloat16*>(out);
-    g.out_stride = out_stride;
-    return (int)LTXATTN_OK;
+    return piece_map(&g.out, out, rows, cols, out_stride, on);
   };
   if (int rc = weight(dgate, a->inner, a->inner, a->x, a->x_stride, a->hidden, a->dw_gate, a->dw_gate_stride,
-                      "workspace", "x"))
+                      "workspace", "x", "dw_gate"))
     return rc;
-  if (int rc = weight(dup, a->inner, a->inner, a->x, a->x_stride, a->hidden, a->dw_up, a->dw_up_stride, "workspace", "x"))
+  if (int rc = weight(dup, a->inner, a->inner, a->x, a->x_stride, a->hidden, a->dw_up, a->dw_up_stride, "workspace", "x",
+                      "dw_up"))
     return rc;
   if (int rc = weight(a->dout, a->dout_stride, a->out_dim, h, a->inner, a->inner, a->dw_down, a->dw_down_stride, "dout",
-                      "workspace"))
+                      "workspace", "dw_down"))
     return rc;
   if (p.count == 0) return LTXATTN_OK;
   return launch_gemm<true, true, kStore>(p, 4, call, st);
