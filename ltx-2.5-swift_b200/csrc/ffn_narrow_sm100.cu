@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
   const uint32_t partial = smem_u32(sm);
   const int n_tokens = min(p.columns, p.tokens - t0);
   const bool have = warp_wait(acc_full, 0, abort_flag, p.err, 67);
+  grid_dep_wait();  // over by now: for these threads too, what was written before is visible
   tc_fence_after();
   // TMEM is read 16 columns at a time: pieces start at multiples of 16, so that none reads past p.columns
   const int piece = n_tokens <= kExchange<kMode> ? kExchange<kMode> : kExchange<kMode> / 16 * 16;

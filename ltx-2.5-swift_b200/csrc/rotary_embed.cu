@@ -214,6 +214,8 @@ struct Slot {
 template <typename T, int kP, bool kInterleaved>
 __global__ void __launch_bounds__(kRThreads, 5) rotary_embed_kernel(const __grid_constant__ RotaryEmbedParams p) {
   extern __shared__ float2 turns[];  // [token_lanes][pairs]: (cos, sin), with the magnitude
+  grid_dep_wait();  // all that is read may have been written by the kernel before
+  grid_dep_launch_dependents();
   const int row0 = blockIdx.x * p.token_lanes;
   const int n_rows = min(p.token_lanes, p.rows - row0);
   {
@@ -256,6 +258,8 @@ __global__ void __launch_bounds__(kRThreads, 5) rotary_embed_kernel(const __grid
 // heads the two are even, at 64 this one is slower (185 us against 152).
 template <typename T, int kP, bool kInterleaved>
 __global__ void __launch_bounds__(kRThreads, 5) rotary_embed_few_heads_kernel(const __grid_constant__ RotaryEmbedParams p) {
+  grid_dep_wait();  // all that is read may have been written by the kernel before
+  grid_dep_launch_dependents();
   const unsigned i = blockIdx.x * kRThreads + threadIdx.x, row = i / p.slots, slot = i - row * p.slots;
   if (row >= (unsigned)p.rows) return;
   const int b = row / p.T, t = row - b * p.T;
@@ -283,22 +287,16 @@ int fail_rotary(int status, const char* fmt, ...) {
 }
 
 template <typename T, int kP>
-void launch(const RotaryEmbedParams& p, bool interleaved, cudaStream_t st) {
+cudaError_t launch(const RotaryEmbedParams& p, bool interleaved, cudaStream_t st) {
   if (p.few_heads) {
     const unsigned grid = (unsigned)((int64_t(p.rows) * p.slots + kRThreads - 1) / kRThreads);
-    if (interleaved)
-      rotary_embed_few_heads_kernel<T, kP, true><<<grid, kRThreads, 0, st>>>(p);
-    else
-      rotary_embed_few_heads_kernel<T, kP, false><<<grid, kRThreads, 0, st>>>(p);
-    return;
+    return launch_pdl(interleaved ? rotary_embed_few_heads_kernel<T, kP, true> : rotary_embed_few_heads_kernel<T, kP, false>,
+                      grid, kRThreads, 0, st, p);
   }
   const dim3 grid((unsigned)((p.rows + (int64_t)p.token_lanes - 1) / p.token_lanes), (unsigned)p.head_groups);
   const int threads = p.slot_lanes * p.head_lanes * p.token_lanes;
-  const size_t smem = sizeof(float2) * p.token_lanes * p.pairs;
-  if (interleaved)
-    rotary_embed_kernel<T, kP, true><<<grid, threads, smem, st>>>(p);
-  else
-    rotary_embed_kernel<T, kP, false><<<grid, threads, smem, st>>>(p);
+  return launch_pdl(interleaved ? rotary_embed_kernel<T, kP, true> : rotary_embed_kernel<T, kP, false>, grid, threads,
+                    sizeof(float2) * p.token_lanes * p.pairs, st, p);
 }
 
 // Whether every row of the view starts on a multiple of `elements` elements.  The
@@ -457,22 +455,25 @@ int ltxattn_rotary_embed(const ltxattn_rotary_embed_args* a, void* stream) {
   p.head_groups = (int)std::min<int64_t>({148 * 1024 / threads, (std::max(H, Hk) + p.head_lanes - 1) / p.head_lanes, 65535});
   p.token_lanes = std::max(1, kTargetThreads / (p.slot_lanes * p.head_lanes));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
   if (bf16) {
     switch (kp) {
-      case 8: launch<__nv_bfloat16, 8>(p, il, st); break;
-      case 4: launch<__nv_bfloat16, 4>(p, il, st); break;
-      case 2: launch<__nv_bfloat16, 2>(p, il, st); break;
-      default: launch<__nv_bfloat16, 1>(p, il, st); break;
+      case 8: e = launch<__nv_bfloat16, 8>(p, il, st); break;
+      case 4: e = launch<__nv_bfloat16, 4>(p, il, st); break;
+      case 2: e = launch<__nv_bfloat16, 2>(p, il, st); break;
+      default: e = launch<__nv_bfloat16, 1>(p, il, st); break;
     }
   } else {
     switch (kp) {
-      case 4: launch<float, 4>(p, il, st); break;
-      case 2: launch<float, 2>(p, il, st); break;
-      default: launch<float, 1>(p, il, st); break;
+      case 4: e = launch<float, 4>(p, il, st); break;
+      case 2: e = launch<float, 2>(p, il, st); break;
+      default: e = launch<float, 1>(p, il, st); break;
     }
   }
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail_rotary(LTXATTN_ERR_CUDA, "ltxattn_rotary_embed: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail_rotary(LTXATTN_ERR_CUDA, "ltxattn_rotary_embed: %s", cudaGetErrorString(e));
+  }
   return LTXATTN_OK;
 }
 

@@ -89,7 +89,8 @@ _NOTHING = (0, 0, 0, 0)
 # into the C struct's bytes: 10 us a call, of which 4 are the launch and 3 the outputs, against 15 with one ctypes
 # object per view.
 def _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k, stream, inverse):
-    _check_cuda("q", q)
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        _check_cuda("q", q)
     shape, dtype, device = q.shape, q.dtype, q.get_device()
     if len(shape) != 4:
         raise Failure.shape("q", shape, "[B, heads, tokens, headDim]")
@@ -99,31 +100,30 @@ def _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k
         _dtype_code(q)
     if order is None:
         raise Failure("arg", f"layout {layout!r} is neither 'half' nor 'interleaved'", _lib.ERR_ARG)
-    _check_cuda("frequencies", frequencies)
-    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
-        raise Failure.shape("frequencies", frequencies.shape, "[rotaryDim / 2] float64, contiguous")
-    if frequencies.get_device() != device:
-        _refuse("frequencies", frequencies, frequencies.shape, torch.float64, device)
+    if not isinstance(frequencies, torch.Tensor) or frequencies.get_device() != device:
+        _refuse("frequencies", frequencies, None, torch.float64, device)
+    pairs = frequencies.shape
+    if frequencies.dtype != torch.float64 or len(pairs) != 1 or not frequencies.is_contiguous():
+        raise Failure.shape("frequencies", pairs, "[rotaryDim / 2] float64, contiguous")
     vq = _view("q", q, shape, dtype, device)
     kv_heads, vk, v_out_k = 0, _NOTHING, _NOTHING
     if k is not None:
-        _check_cuda("k", k)
-        kv_heads = k.shape[1] if k.dim() == 4 else 0
+        k_shape = k.shape if isinstance(k, torch.Tensor) else ()
+        kv_heads = k_shape[1] if len(k_shape) == 4 else 0
         k_shape = (B, kv_heads, T, D)
         vk = _view("k", k, k_shape, dtype, device)
     elif out_k is not None:
         raise Failure("arg", "out_k without k", _lib.ERR_ARG)
     at, bits, at_sb, at_st = 0, 0, 0, 0
     if positions is not None:
-        _check_cuda("positions", positions)
+        if not isinstance(positions, torch.Tensor) or positions.get_device() != device:
+            _refuse("positions", positions, None, None, device)
         kind, at_shape, strides = positions.dtype, positions.shape, positions.stride()
         bits = 64 if kind == torch.int64 else 32
         if bits == 32 and kind != torch.int32:
             raise Failure("dtype", f"positions are {kind}, expected int64 or int32", _lib.ERR_DTYPE)
         if at_shape != (B, T) and at_shape != (T,) and at_shape != (1, T):
             raise Failure.shape("positions", at_shape, f"[{T}] or [1|{B}, {T}]")
-        if positions.get_device() != device:
-            _refuse("positions", positions, at_shape, kind, device)
         at, at_st = positions.data_ptr(), strides[-1]
         if len(at_shape) == 2 and at_shape[0] > 1:
             at_sb = strides[0]
@@ -138,7 +138,7 @@ def _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k
             else:
                 v_out_k = _view("out_k", out_k, k_shape, dtype, device)
         rc = _lib.load().ltxattn_rotary_embed(
-            _lib.ROTARY_EMBED_ARGS.pack(code, B, T, H, kv_heads, D, 2 * frequencies.shape[0], order, inverse, magnitude,
+            _lib.ROTARY_EMBED_ARGS.pack(code, B, T, H, kv_heads, D, 2 * pairs[0], order, inverse, magnitude,
                                         *vq, *v_out_q, *vk, *v_out_k, frequencies.data_ptr(), at, bits, at_sb, at_st,
                                         offset), st)
     if rc != _lib.OK:
