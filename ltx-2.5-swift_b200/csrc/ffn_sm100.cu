@@ -104,8 +104,10 @@ struct GemmParams {
 // ---------------------------------------------------------------------------
 
 // Tiles are numbered down the rows first, in bands of kBand row blocks: the CTAs
-// that run together then share a few column blocks of B and the band's rows of A.
-constexpr int kBand = 8;
+// that run together then share a few column blocks of B and the band's rows of A.  4096 rows: of 3120 tokens the
+// weights are then read once (bands of 1024, 2048 and 4096 rows: 1026, 993 and 979 us for the forward at 4096 x 16384,
+// under the power cap).
+constexpr int kBand = 16;
 
 __device__ __forceinline__ void locate(const GemmParams& p, int tile, int& which, int& m0, int& tn) {
   which = 0;
