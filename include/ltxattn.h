@@ -406,6 +406,7 @@ typedef enum ltxattn_activation {
  *    aligned; hidden, inner and out_dim multiples of 8; any m >= 0.
  *  - gate, up: both NULL, or [m, inner] outputs that keep x w_gate^T and
  *    x w_up^T (rounded to bf16) for the gradient.
+ *  - Outputs must not overlap inputs or one another.
  *  - workspace: ltxattn_gated_ffn_workspace() bytes, 256-byte aligned: the
  *    product act(..) * (..) in bf16 between the two kernels, 2 m inner bytes
  *    rounded up to 256. */

@@ -12,11 +12,11 @@
 // all.  A pair of CTAs (a cluster, cta_group::2) walks over 256 x 256 output
 // tiles: each holds 128 rows of A and 128 of B's 256 columns in its shared
 // memory, and 128 rows of the result in its TMEM, so an SM loads 32 KB for the
-// MMAs that one on its own would load 48 KB for.  In each CTA warp 0 lane 0
-// loads 64-wide K slices with TMA into a ring of stages (128-byte swizzle) that
-// the first CTA's barrier counts; there warp 1 lane 0 issues the MMAs for both;
-// warps 4-11 turn the finished accumulator into the output while the next tile's
-// MMAs fill the other half of TMEM.
+// MMAs that one on its own would load 48 KB for.  In each CTA warps 0 and 2
+// load 64-wide K slices of A and B with TMA into a ring of stages (128-byte
+// swizzle) that the first CTA's barriers count; there warp 1 issues the MMAs for
+// both; warps 4-11 turn the finished accumulator into the output while the next
+// tile's MMAs fill the other half of TMEM.
 //
 // Operands that lie along the wrong axis (the weights of dh and dx, both
 // operands of the weight gradients) are read as they lie: their tiles are
@@ -31,7 +31,12 @@
 // outputs are rounded once.
 //
 // Bound: the tensor cores (at 3120 x 4096 x 16384 the forward does 2770
-// operations per byte it must move).
+// operations per byte it must move).  That forward takes 851 us on a cool GPU
+// (1.48 PFLOP/s, 0.89 of the measured burst rate of a library GEMM) and 976 back
+// to back under the power cap (0.93 of the measured sustained rate; the two bare
+// products in the library: 802 and 942).  The backward takes 1829 and 2100 us
+// (library products alone: 1619 and 1898); the difference is dh's epilogue, whose
+// 640 KB a tile share the shared-memory bandwidth that the MMAs nearly fill.
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
@@ -45,12 +50,12 @@ int set_error_message(int status, const char* msg);
 
 namespace {
 
-constexpr int kGM = 128;       // rows of a CTA's part of a tile
+constexpr int kGM = 128;          // rows of a CTA's part of a tile
 constexpr int kGPairM = 2 * kGM;  // rows of a tile (UMMA M)
-constexpr int kGN = 256;       // accumulator columns of a tile (UMMA N)
+constexpr int kGN = 256;          // accumulator columns of a tile (UMMA N)
 constexpr int kGHalfN = kGN / 2;  // of which a CTA holds the operand
 constexpr int kGK = kFfnK;
-constexpr int kGThreads = 384;  // 4 control warps, 8 epilogue warps
+constexpr int kGThreads = 384;    // 4 control warps, 8 epilogue warps
 constexpr uint32_t kGA = kGM * kGK * 2;
 constexpr uint32_t kGB = kGHalfN * kGK * 2;
 constexpr uint32_t kGStage = kGA + kGB;
@@ -540,6 +545,15 @@ int check_mat(const char* call, const Mat& m) {
   return LTXATTN_OK;
 }
 
+// Refuses an output (from `first` on) that is another of the call's matrices.
+int check_distinct(const char* call, const Mat* mats, int count, int first) {
+  for (int i = first; i < count; ++i)
+    for (int j = 0; j < i; ++j)
+      if (mats[i].data != nullptr && mats[i].data == mats[j].data)
+        return fail_ffn(LTXATTN_ERR_ARG, "%s: %s and %s are the same memory", call, mats[j].name, mats[i].name);
+  return LTXATTN_OK;
+}
+
 int check_sizes(const char* call, int dtype, int activation, int m, int hidden, int inner, int out_dim) {
   if (dtype != LTXATTN_BF16) return fail_ffn(LTXATTN_ERR_DTYPE, "%s: bf16 only", call);
   if (activation < LTXATTN_SILU || activation > LTXATTN_GELU)
@@ -660,6 +674,7 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
                        {"up", a->up, a->up_stride, a->m, a->inner}};
   for (int i = 0; i < (a->gate ? 7 : 5); ++i)
     if (int rc = check_mat(call, mats[i])) return rc;
+  if (int rc = check_distinct(call, mats, 7, 4)) return rc;
   if (int rc = check_workspace(call, a->workspace, a->workspace_bytes, ltxattn_gated_ffn_workspace(a))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   __nv_bfloat16* h = static_cast<__nv_bfloat16*>(a->workspace);
@@ -763,6 +778,10 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     if (i == 6 && !dw_in) continue;
     if (int rc = check_mat(call, ins[i])) return rc;
   }
+  Mat all[11];
+  std::copy(ins, ins + 7, all);
+  std::copy(outs, outs + 4, all + 7);
+  if (int rc = check_distinct(call, all, 11, 7)) return rc;
   if (int rc = check_workspace(call, a->workspace, a->workspace_bytes, ltxattn_gated_ffn_bwd_workspace(a))) return rc;
   const size_t plane = plane_bytes(a->m, a->inner);
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);

@@ -411,6 +411,9 @@ int ltxattn_rotary_embed(const ltxattn_rotary_embed_args* a, void* stream) {
   if (Hk > 0)
     if (int rc = check_view("k", a->k, a->k_out, B, Hk, T, size)) return rc;
 
+  if (H > 0 && Hk > 0 && (a->q_out.data == a->k_out.data || a->q_out.data == a->k.data || a->k_out.data == a->q.data))
+    return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_embed: an output of q or k is the other's memory");
+
   RotaryEmbedParams p{};
   p.pairs = a->rotary_dim / 2;
   // kP: as many pairs to a slot as give runs of 16 bytes (half) or 32 (interleaved) at most, of which the pairs, the

@@ -8,12 +8,13 @@ Tolerances are bounds, element by element, carried through the formulas from
    units of 2^-24 each, over arguments of a few tens), relative to their size.
 A tensor's bound is returned beside it by `forward` and `backward` below.
 """
+import ctypes
 import math
 
 import pytest
 import torch
 
-from ltxattn import (AttentionBackend, device_status, gated_ffn, gated_ffn_backward, linear, rotary_embed,
+from ltxattn import (AttentionBackend, _lib, device_status, gated_ffn, gated_ffn_backward, linear, rotary_embed,
                      rotary_embed_backward, rotary_frequencies)
 
 pytestmark = pytest.mark.gpu
@@ -195,6 +196,42 @@ def test_views_and_batches():
                        dw_up=stacked[inner:2 * inner])
     assert torch.equal(stacked[:inner], got[1]) and torch.equal(stacked[inner:-1], got[2])
     assert bool((stacked[-1] == 5).all())
+
+
+@pytest.mark.parametrize("m", [20, 300])
+@pytest.mark.parametrize("which", ["dx", "dw_gate", "dw_up", "dw_down"])
+def test_single_gradients_through_the_c_entry(m, which):
+    # each output alone, with the inputs that only the others read left out
+    hidden, inner, out = 64, 200, 72
+    x, wg, wu, wd, dout = make(13, m, hidden, inner, out)
+    _, gate, up = gated_ffn(x, wg, wu, wd, save=True)
+    want = dict(zip(("dx", "dw_gate", "dw_up", "dw_down"), gated_ffn_backward(x, wg, wu, wd, gate, up, dout)))[which]
+    a = _lib.GatedFfnBwdArgs(_lib.BF16, 0, m, hidden, inner, out)
+    got = torch.full_like(want, 7.0)
+    given = dict(gate=gate, up=up, dout=dout, w_down=wd)
+    given |= {"dx": dict(w_gate=wg, w_up=wu), "dw_down": {}}.get(which, dict(x=x))
+    for name, t in {**given, which: got}.items():
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_stride", t.stride(0))
+    L = _lib.load()
+    ws = torch.empty(L.ltxattn_gated_ffn_bwd_workspace(ctypes.byref(a)), dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    assert L.ltxattn_gated_ffn_bwd(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == _lib.OK, _lib.last_error()
+    assert torch.equal(got, want)
+
+
+def test_rows_past_32_bits():
+    # 140 thousand tokens of 16384: the planes between the kernels have 2.3e9 elements
+    m, hidden, inner, out = 140001, 64, 16384, 72
+    x, wg, wu, wd, dout = make(14, m, hidden, inner, out)
+    tail = slice(m - 300, m)
+    want, want_gate, want_up = forward(x[tail], wg, wu, wd, "silu")
+    y, gate, up = gated_ffn(x, wg, wu, wd, save=True)
+    check("y", y[tail], want)
+    check("gate", gate[tail], want_gate)
+    check("up", up[tail], want_up)
+    dx, *_ = gated_ffn_backward(None, wg, wu, wd, gate, up, dout, need_dw=False)
+    check("dx", dx[tail], backward(x[tail], wg, wu, wd, gate[tail], up[tail], dout[tail], "silu")[0])
 
 
 def test_no_tokens():

@@ -144,6 +144,20 @@ def test_in_place_and_views(layout, rot):
     check(rotary_embed(shared, freq, layout=layout), shared, freq, row(B, T), layout)
 
 
+def test_cache_slots_past_32_bits():
+    # two heads 2^31 elements apart: the offsets of the second need 64 bits
+    slots, T, D = 2 ** 24 + 64, 40, 128
+    cache = torch.empty((1, 2, slots, D), dtype=torch.bfloat16, device="cuda")
+    cache[:, :, -T - 1] = 3.0
+    q = heads(16, 1, T, 2, D, torch.bfloat16)
+    freq, _ = rotary_frequencies(D)
+    rotary_embed(q, freq, offset=slots - T, out_q=cache[:, :, -T:])
+    check(cache[:, :, -T:], q, freq, row(1, T, slots - T), "half")
+    assert bool((cache[:, :, -T - 1] == 3).all())
+    # and read from there
+    check(rotary_embed(cache[:, :, -T:], freq), cache[:, :, -T:], freq, row(1, T), "half")
+
+
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_backward_is_the_transpose(layout, dtype):

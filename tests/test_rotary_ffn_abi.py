@@ -161,6 +161,8 @@ def rotary_args(**kw):
     ({"q_out.stride_t": 0}, _lib.ERR_SHAPE),   # an output that repeats rows
     ({"q_out.stride_h": 0}, _lib.ERR_SHAPE),
     ({"q_out.data": 4096, "q_out.stride_t": 64}, _lib.ERR_ARG),  # in place with other strides
+    ({"q_out.data": 4096 * 4}, _lib.ERR_ARG),  # both outputs in one place
+    ({"k_out.data": 4096}, _lib.ERR_ARG),      # keys over the queries
 ])
 def test_rotary_refusals(kw, status):
     L = _lib.load()
@@ -226,8 +228,10 @@ BOTH = [
 
 @pytest.mark.parametrize("kw,status", BOTH + [
     (dict(out=None), _lib.ERR_ARG),
-    (dict(gate=4096, gate_stride=128), _lib.ERR_ARG),                              # gate without up
-    (dict(gate=4096, gate_stride=64, up=8192, up_stride=128), _lib.ERR_SHAPE),
+    (dict(gate=1 << 16, gate_stride=128), _lib.ERR_ARG),                             # gate without up
+    (dict(gate=1 << 16, gate_stride=64, up=1 << 17, up_stride=128), _lib.ERR_SHAPE),
+    (dict(gate=1 << 16, gate_stride=128, up=1 << 16, up_stride=128), _lib.ERR_ARG),  # gate and up in one place
+    (dict(out=4096, out_stride=72), _lib.ERR_ARG),                                   # y over x
 ])
 def test_ffn_refusals(kw, status):
     rc = _lib.load().ltxattn_gated_ffn(ctypes.byref(ffn_args(**kw)), None)
@@ -240,6 +244,8 @@ def test_ffn_refusals(kw, status):
     (dict(dout=4104), _lib.ERR_ALIGN),
     (dict(dx_stride=8), _lib.ERR_SHAPE),
     (dict(dw_down=4097), _lib.ERR_ALIGN),
+    (dict(dx=4096), _lib.ERR_ARG),              # dx over x
+    (dict(dw_up=4096 * 9), _lib.ERR_ARG),       # over dw_gate
 ])
 def test_ffn_backward_refusals(kw, status):
     rc = _lib.load().ltxattn_gated_ffn_bwd(ctypes.byref(bwd_args(**kw)), None)
