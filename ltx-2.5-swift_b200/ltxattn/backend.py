@@ -153,11 +153,11 @@ class _on:
             self.guard = torch.cuda.stream(self.stream)
             self.guard.__enter__()
             return self.stream.cuda_stream
-        if torch.cuda.current_device() != self.device:
+        if torch._C._cuda_getDevice() != self.device:
             self.guard = torch.cuda.device(self.device)
             self.guard.__enter__()
-        # the handle that torch.cuda.current_stream(device).cuda_stream gives, without making the
-        # stream object (3 us, a third of a small call)
+        # what torch.cuda.current_device() and torch.cuda.current_stream(device).cuda_stream give, without
+        # making the stream object (3 us, a third of a small call)
         return torch._C._cuda_getCurrentRawStream(self.device)
 
     def __exit__(self, *exc):

@@ -55,9 +55,9 @@ def _output(name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor):
 
 
 def _planes(n: int, m: int, inner: int, like: torch.Tensor) -> torch.Tensor:
-    """A workspace of n bf16 [m, inner] planes, as ltxattn_gated_ffn_workspace counts them (asking it would take
-    another packing of the arguments)."""
-    return like.new_empty((n * ((2 * m * inner + 255) // 256 * 256),), dtype=torch.uint8)
+    """A workspace of n bf16 [m, inner] planes, each rounded up to 256 bytes, as ltxattn_gated_ffn_workspace counts
+    them (asking it would take another packing of the arguments).  ``like`` is bf16."""
+    return like.new_empty(n * ((2 * m * inner + 255) // 256 * 128))
 
 
 def _out_rows(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -121,7 +121,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
                 *((y.data_ptr(), out_dim) if out is None else _matrix("out", _out_rows("out", y), m, out_dim, device)),
                 *kept)
         ws = _planes(1, m, inner, x)
-        rc = _lib.load().ltxattn_gated_ffn(_lib.GATED_FFN_ARGS.pack(*args, ws.data_ptr(), ws.numel()), st)
+        rc = _lib.load().ltxattn_gated_ffn(_lib.GATED_FFN_ARGS.pack(*args, ws.data_ptr(), 2 * ws.numel()), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
     return (y, gate, up) if save else y
@@ -178,7 +178,7 @@ def gated_ffn_backward(x: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: to
                 *_matrix("w_gate", w_gate, inner, hidden, device), *_matrix("w_up", w_up, inner, hidden, device),
                 *_matrix("w_down", w_down, out_dim, inner, device), *_matrix("gate", gate2, m, inner, device),
                 *_matrix("up", up2, m, inner, device), *_matrix("dout", d2, m, out_dim, device), *to[0], *to[1],
-                *to[2], *to[3], ws.data_ptr(), ws.numel()), st)
+                *to[2], *to[3], ws.data_ptr(), 2 * ws.numel()), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
     return (dx if need_dx else None,) + ((dw_gate, dw_up, dw_down) if need_dw else (None, None, None))

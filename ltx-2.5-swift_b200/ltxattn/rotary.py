@@ -105,7 +105,9 @@ def _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k
     pairs = frequencies.shape
     if frequencies.dtype != torch.float64 or len(pairs) != 1 or not frequencies.is_contiguous():
         raise Failure.shape("frequencies", pairs, "[rotaryDim / 2] float64, contiguous")
-    vq = _view("q", q, shape, dtype, device)
+    q_sb, q_sh, q_st, unit = q.stride()
+    if unit != 1:
+        _refuse("q", q, shape, dtype, device)
     kv_heads, vk, v_out_k = 0, _NOTHING, _NOTHING
     if k is not None:
         k_shape = k.shape if isinstance(k, torch.Tensor) else ()
@@ -139,8 +141,8 @@ def _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k
                 v_out_k = _view("out_k", out_k, k_shape, dtype, device)
         rc = _lib.load().ltxattn_rotary_embed(
             _lib.ROTARY_EMBED_ARGS.pack(code, B, T, H, kv_heads, D, 2 * pairs[0], order, inverse, magnitude,
-                                        *vq, *v_out_q, *vk, *v_out_k, frequencies.data_ptr(), at, bits, at_sb, at_st,
-                                        offset), st)
+                                        q.data_ptr(), q_sb, q_sh, q_st, *v_out_q, *vk, *v_out_k,
+                                        frequencies.data_ptr(), at, bits, at_sb, at_st, offset), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
     return out_q if k is None else (out_q, out_k)
