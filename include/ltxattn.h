@@ -370,8 +370,9 @@ LTXATTN_API int ltxattn_rotary_frequencies(const ltxattn_rotary_frequency_args* 
  *    token t stands at t.  `offset` is added to each position.
  *  - inverse: turn the other way; with the same magnitude this is the gradient
  *    (the transpose) of the call without it.
- * Angles are formed and reduced to an eighth of a turn in fp64; cos and sin of
- * the rest and the products are fp32, and each element is rounded once. */
+ * Angles are formed and reduced to an eighth of a turn in fp64 (position + offset
+ * and its angle must stay below 2^51 in size); cos and sin of the rest and the
+ * products are fp32, and each element is rounded once. */
 typedef struct ltxattn_rotary_embed_args {
   int32_t dtype;
   int32_t batch, tokens, heads, kv_heads, head_dim;

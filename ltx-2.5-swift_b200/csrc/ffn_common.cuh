@@ -15,7 +15,8 @@ namespace ltx {
 // ---------------------------------------------------------------------------
 // activations (fp32)
 
-// The fast division is off by 2 units of 2^-24; 1 + e^-x is at most infinite, and then it gives 0.
+// The fast division is off by 2 units of 2^-24, and gives 0 for a divisor above 2^126: there, for x < -87, the sigmoid
+// is below 2^-126 and 0 is as near as bf16 products need.
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
 // act(g), and with kSlope its derivative too.

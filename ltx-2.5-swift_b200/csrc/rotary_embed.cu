@@ -36,6 +36,7 @@ constexpr int kRThreads = 256;      // of a CTA at most
 constexpr int kFewHeads = 16;        // q's and k's together
 constexpr int kTargetThreads = 128;  // slots x head lanes, where the slots alone are fewer
 constexpr int kMaxRotaryDim = 8192;
+constexpr int kMaxHeads = 1 << 24;   // heads are counted in 32 bits, several steps ahead
 
 struct RView {
   const void* x;
@@ -397,6 +398,8 @@ int ltxattn_rotary_embed(const ltxattn_rotary_embed_args* a, void* stream) {
   if (a->rotary_dim > kMaxRotaryDim)
     return fail_rotary(LTXATTN_ERR_UNSUPPORTED, "ltxattn_rotary_embed: rotary_dim (%d) is above %d", a->rotary_dim,
                        kMaxRotaryDim);
+  if (H > kMaxHeads || Hk > kMaxHeads)
+    return fail_rotary(LTXATTN_ERR_UNSUPPORTED, "ltxattn_rotary_embed: more than %d heads", kMaxHeads);
   if (B == 0 || T == 0 || H + Hk == 0) return LTXATTN_OK;
   if (a->frequencies == nullptr) return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_embed: frequencies is required");
   if (reinterpret_cast<uintptr_t>(a->frequencies) % 8 ||

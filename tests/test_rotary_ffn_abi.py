@@ -154,6 +154,8 @@ def rotary_args(**kw):
     (dict(positions=4096, position_stride_t=-1), _lib.ERR_SHAPE),
     (dict(head_dim=16384, rotary_dim=16384), _lib.ERR_UNSUPPORTED),
     (dict(tokens=2 ** 30), _lib.ERR_UNSUPPORTED),
+    (dict(heads=2 ** 24 + 1), _lib.ERR_UNSUPPORTED),  # steps through the heads are counted in 32 bits
+    (dict(kv_heads=2 ** 24 + 1), _lib.ERR_UNSUPPORTED),
     ({"q.data": None}, _lib.ERR_ARG),
     ({"k_out.data": None}, _lib.ERR_ARG),
     ({"q.data": 4097}, _lib.ERR_ALIGN),
