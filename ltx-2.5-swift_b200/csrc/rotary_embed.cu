@@ -48,7 +48,7 @@ struct RView {
 
 struct RotaryEmbedParams {
   RView v[2];  // q, k
-  int T, pairs;
+  int T, pairs, head_dim;
   int rows;          // B * T
   int slots;         // slots of a token: turned ones, then copied ones
   int turn_slots;    // pairs / kP
@@ -150,7 +150,8 @@ __device__ __forceinline__ double place(const RotaryEmbedParams& p, int b, int t
 // How a slot lies in a head.  kP pairs per turned slot: two runs of kP elements,
 // `pairs` apart, in the half layout, one run of 2 kP in the interleaved one (a
 // single interleaved pair is two runs of one element: its row may start
-// anywhere).  Copied slots are one run.
+// anywhere).  Copied slots are as many runs, side by side; where their number is odd the last slot moves its run
+// twice.  With one run to a copied slot, 6242 fp32 tokens x 36 heads x 64, 24 of them turned, took 28 us for 22.
 template <typename T, int kP, bool kInterleaved>
 struct Slot {
   static constexpr bool kTwoRuns = !kInterleaved || kP == 1;
@@ -161,8 +162,9 @@ struct Slot {
 
   __device__ __forceinline__ Slot(const RotaryEmbedParams& p, int slot)
       : turned(slot < p.turn_slots),
-        at(turned ? (kInterleaved ? 2 * kP : kP) * slot : 2 * p.pairs + kRun * (slot - p.turn_slots)),
-        apart(kInterleaved ? 1 : p.pairs) {}
+        at(turned ? (kInterleaved ? 2 * kP : kP) * slot
+                  : 2 * p.pairs + (kTwoRuns ? 2 : 1) * kRun * (slot - p.turn_slots)),
+        apart(turned && !kInterleaved ? p.pairs : at + 2 * kRun <= p.head_dim ? kRun : 0) {}
 
   // through the heads h, h + step, ... of a view's token; short runs take several heads at once, to have as many
   // bytes on their way as a long one
@@ -180,7 +182,7 @@ struct Slot {
       for (int u = 0; u < kAtOnce; ++u) {
         if (u > 0 && h + u * step >= v.heads) break;
         r0[u] = load_run<R>(x + u * dx);
-        if (kTwoRuns && turned) r1[u] = load_run<R>(x + u * dx + apart);
+        if (kTwoRuns) r1[u] = load_run<R>(x + u * dx + apart);
       }
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
@@ -194,8 +196,8 @@ struct Slot {
             from_f(ea, fmaf(fa, c[e], -(fb * s[e])));
             from_f(eb, fmaf(fb, c[e], fa * s[e]));
           }
-          if (kTwoRuns) store_run(y + u * dy + apart, r1[u]);
         }
+        if (kTwoRuns) store_run(y + u * dy + apart, r1[u]);
         store_run(y + u * dy, r0[u]);
       }
     }
@@ -443,7 +445,8 @@ int ltxattn_rotary_embed(const ltxattn_rotary_embed_args* a, void* stream) {
   if (B * T > 0x7fffffff) return fail_rotary(LTXATTN_ERR_UNSUPPORTED, "ltxattn_rotary_embed: too many tokens for one call");
   p.rows = (int)(B * T);
   p.turn_slots = p.pairs / kp;
-  p.slots = p.turn_slots + (in_place ? 0 : (a->head_dim - a->rotary_dim) / (il && kp > 1 ? 2 * kp : kp));
+  p.head_dim = a->head_dim;
+  p.slots = p.turn_slots + (in_place ? 0 : (a->head_dim - a->rotary_dim + 2 * kp - 1) / (2 * kp));
   p.freq = a->frequencies;
   p.positions = a->positions;
   p.pos64 = a->position_bits == 64;

@@ -66,6 +66,8 @@ def row(B, T, offset=0):
     (2, 20000, 2, 1, 64, 64),    # many tokens of few heads: a thread through all heads of a token
     (1, 30011, 3, 2, 40, 24),
     (3, 9001, 1, 1, 37, 6),
+    (2, 41, 9, 2, 76, 24),       # what is copied is an odd number of runs
+    (1, 12007, 6, 2, 76, 24),
 ])
 def test_matches_the_rotation(layout, dtype, B, T, H, Hk, D, rot):
     q, k = heads(1, B, T, H, D, dtype), heads(2, B, T, Hk, D, dtype)
