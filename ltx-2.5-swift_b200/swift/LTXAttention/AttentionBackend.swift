@@ -195,6 +195,90 @@ public enum AttentionBackend {
         try check(ltxattn_rotary_tables(&a, stream))
     }
 
+    /// How `rotaryFrequencies` stretches the pairs for contexts beyond the trained one
+    /// (ltxattn_rotary_scaling).
+    public enum RotaryScaling {
+        case none
+        case linear(factor: Double)
+        case ntk(factor: Double)
+        case yarn(factor: Double, trainedLength: Double, fast: Double, slow: Double)
+        case bands(factor: Double, trainedLength: Double, fast: Double, slow: Double)
+    }
+
+    /// The angle of each pair per position (host memory, to be copied to the device once) and the
+    /// factor on what is turned, for `rotaryEmbed`.
+    public static func rotaryFrequencies(
+        rotaryDim: Int32, theta: Double, scaling: RotaryScaling = .none
+    ) throws -> (frequencies: [Double], magnitude: Float) {
+        var a = ltxattn_rotary_frequency_args()
+        a.rotary_dim = rotaryDim; a.theta = theta
+        switch scaling {
+        case .none:
+            a.scaling = Int32(LTXATTN_ROTARY_NONE.rawValue)
+        case .linear(let factor):
+            a.scaling = Int32(LTXATTN_ROTARY_LINEAR.rawValue); a.factor = factor
+        case .ntk(let factor):
+            a.scaling = Int32(LTXATTN_ROTARY_NTK.rawValue); a.factor = factor
+        case .yarn(let factor, let length, let fast, let slow):
+            a.scaling = Int32(LTXATTN_ROTARY_YARN.rawValue)
+            a.factor = factor; a.trained_length = length; a.fast = fast; a.slow = slow
+        case .bands(let factor, let length, let fast, let slow):
+            a.scaling = Int32(LTXATTN_ROTARY_BANDS.rawValue)
+            a.factor = factor; a.trained_length = length; a.fast = fast; a.slow = slow
+        }
+        var frequencies = [Double](repeating: 0, count: max(1, Int(rotaryDim) / 2))
+        var magnitude: Float = 1
+        try check(ltxattn_rotary_frequencies(&a, &frequencies, &magnitude))
+        return (frequencies, magnitude)
+    }
+
+    /// Rotary positions from token indices, for q [B, heads, T, D] and k [B, kvHeads, T, D] in one
+    /// launch (the rotation before a grouped-head attention, GemmaTextEncoder.swift:173,193);
+    /// `inverse` takes gradients back.  `positions` is [B, T] int64 on the device with the given
+    /// element strides, nil for 0, 1, 2, ...; `offset` is added to each.
+    public static func rotaryEmbed(
+        bf16: Bool, batch: Int32, tokens: Int32, heads: Int32, kvHeads: Int32, headDim: Int32,
+        rotaryDim: Int32, interleaved: Bool, magnitude: Float, frequencies: UnsafePointer<Double>,
+        q: DeviceTensor, qOut: DeviceTensor, k: DeviceTensor? = nil, kOut: DeviceTensor? = nil,
+        positions: UnsafePointer<Int64>? = nil, positionStrides: (b: Int64, t: Int64) = (0, 1),
+        offset: Int64 = 0, inverse: Bool = false, stream: UnsafeMutableRawPointer?
+    ) throws {
+        var a = ltxattn_rotary_embed_args()
+        a.dtype = bf16 ? Int32(LTXATTN_BF16.rawValue) : Int32(LTXATTN_F32.rawValue)
+        a.batch = batch; a.tokens = tokens; a.heads = heads; a.head_dim = headDim
+        a.rotary_dim = rotaryDim
+        a.layout = Int32((interleaved ? LTXATTN_ROTARY_INTERLEAVED : LTXATTN_ROTARY_HALF).rawValue)
+        a.inverse = inverse ? 1 : 0
+        a.magnitude = magnitude
+        a.q = q.c; a.q_out = qOut.c
+        if let k, let kOut { a.kv_heads = kvHeads; a.k = k.c; a.k_out = kOut.c }
+        a.frequencies = frequencies
+        a.positions = UnsafeRawPointer(positions); a.position_bits = 64
+        a.position_stride_b = positionStrides.b; a.position_stride_t = positionStrides.t
+        a.offset = offset
+        try check(ltxattn_rotary_embed(&a, stream))
+    }
+
+    /// The gated feed-forward block of prepared arguments; `gatedFFNWorkspaceBytes` sizes its
+    /// workspace (call once per shape; the caller allocates).
+    public static func gatedFFN(_ a: inout ltxattn_gated_ffn_args, stream: UnsafeMutableRawPointer?) throws {
+        try check(ltxattn_gated_ffn(&a, stream))
+    }
+
+    public static func gatedFFNWorkspaceBytes(_ a: inout ltxattn_gated_ffn_args) -> Int {
+        Int(ltxattn_gated_ffn_workspace(&a))
+    }
+
+    /// The gradients of the block's input and weights, each where its pointer is set.
+    public static func gatedFFNBackward(_ a: inout ltxattn_gated_ffn_bwd_args,
+                                        stream: UnsafeMutableRawPointer?) throws {
+        try check(ltxattn_gated_ffn_bwd(&a, stream))
+    }
+
+    public static func gatedFFNBackwardWorkspaceBytes(_ a: inout ltxattn_gated_ffn_bwd_args) -> Int {
+        Int(ltxattn_gated_ffn_bwd_workspace(&a))
+    }
+
     /// The q / k preparation of DiTAttention.swift:358-367 in one pass: rmsNorm over the
     /// inner dim, the head split and split RoPE, from the projection output
     /// [B, tokens, heads * headDim] (element strides `xStrides`) into `out`.
