@@ -105,6 +105,12 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
+// The same without an order on memory.
+__device__ __forceinline__ void cluster_barrier_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  asm volatile("barrier.cluster.wait;" ::: "memory");
+}
+
 // The address that `local` has in this CTA, of the CTA with that rank (shared::cluster window).
 __device__ __forceinline__ uint32_t peer_address(uint32_t local, uint32_t rank) {
   uint32_t at;
