@@ -344,34 +344,38 @@ int launch(NarrowParams& p, bool follows, const char* call, cudaStream_t st) {
 // some of the 296 places empty.
 constexpr int kPlaces[kNMaxCluster + 1] = {0, 296, 296, 270, 264, 260, 264, 210, 240};
 
-// What a cut takes, in microseconds: 2.5 a product and 3 a round of CTAs; an SM brings in 1 KB of a K slice per 10
-// ns, and 1 KB of another CTA's sums per 28 ns, for the one or two CTAs that it holds; and all weights come in at 6.4
+// What a cut takes, in microseconds: 1.5 a product and 3 a round of CTAs; an SM brings in 1 KB of a K slice per 10
+// ns, and 1 KB of another CTA's sums per 28 ns, and finishes a token's 128 features in 50 ns (30 for a gradient, next to
+// nothing for a plain store), for the one or two CTAs that it holds; and all weights come in at 6.4
 // TB/s, which takes the loads of 256 CTAs in flight (19 tokens at 2048 x 8192 with 128, 192 and 256 CTAs for the first
 // product: 32.3, 29.1 and 28.5 us for both).  Fitted to 2700 cuts of 128 products (96 to 1024 tokens, 1024 to 16384
-// features): the cut that it finds fastest is 0.8 us slower than the fastest one measured, on average.
-double cut_us(int parts, int tokens, int features, int kb, int columns, int cluster) {
+// features): the cut that it finds fastest is 0.8 us slower than the fastest one measured, on average.  The time to finish a token
+// was fitted to 70 calls by both kernels (47 to 720 tokens).
+double cut_us(NarrowMode mode, int tokens, int features, int kb, int columns, int cluster) {
+  const int parts = mode == kNarrowProduct ? 2 : 1;
+  const double finish = mode == kNarrowProduct ? 0.05 : mode == kNarrowSlopes ? 0.03 : 0.0;  // of a token
   const int64_t ctas = div_up(features, kNRows) * div_up(tokens, columns) * cluster;
   const int64_t rounds = ctas / kPlaces[cluster], rest = ctas - rounds * kPlaces[cluster];
   const double cta = 0.0103 * div_up(kb, cluster) * (parts * 16 + columns / 8.0) +
                      0.0285 * columns * parts * 0.5 * (cluster - 1) / cluster +
-                     (cluster > 1 && columns * parts > 208 ? 1.5 : 0.0);  // the exchange in two pieces
-  double us = 2.5 + rounds * (3.0 + 2 * cta);
+                     (cluster > 1 && columns * parts > 208 ? 1.5 : 0.0) +  // the exchange in two pieces
+                     finish * columns / cluster;
+  double us = 1.5 + rounds * (3.0 + 2 * cta);
   if (rest > 0) us += 3.0 + cta * (rest > 148 ? 2.0 : 1.0 + rest / 148.0);
   const double idle = std::max(0.0, (256.0 - ctas) / 128);
-  return std::max(us, 5.5 + 2e-5 * features * parts * kb * (1 + 0.28 * idle * idle));
+  return std::max(us, 4.5 + 2e-5 * features * parts * kb * (1 + 0.28 * idle * idle));
 }
 
 // The fastest cut: token tiles as few as fit (128 columns each) or up to three more, 1 to 8 CTAs to a tile with a
 // K slice each.  More token tiles exchange less but load the weights more often from L2; more CTAs to a tile keep
 // more loads in flight but exchange more.
 NarrowPlan plan_narrow(NarrowMode mode, int tokens, int features, int kb) {
-  const int parts = mode == kNarrowProduct ? 2 : 1;
   const int64_t least = div_up(tokens, kNarrowColumns);
   NarrowPlan best{0, 0, 0};
   for (int64_t t = least; t <= least + 3; ++t) {
     const int columns = (int)div_up(div_up(tokens, t), 16) * 16;
     for (int s = 1; s <= std::min(kNMaxCluster, kb); ++s) {
-      const double us = cut_us(parts, tokens, features, kb, columns, s);
+      const double us = cut_us(mode, tokens, features, kb, columns, s);
       if (best.cluster == 0 || us < best.us) best = {columns, s, us};
     }
     if (columns == 16) break;

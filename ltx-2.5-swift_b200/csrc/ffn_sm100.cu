@@ -618,13 +618,14 @@ int launch_gemm(GemmParams& p, int slot, const char* call, cudaStream_t st) {
 }
 
 // Whether a product runs feature by feature (ffn_narrow_sm100.cu), by what both kernels were measured to take.  The
-// wide kernel pays for rounds of tiles over 74 CTA pairs, which few tokens leave mostly empty.  Over 164 calls (24 to
-// 2000 tokens, 256 to 16384 features, both directions) the choice was 0.5% slower than the best of both kernels for
-// each product, on average; choosing by 128, 256 and 512 tokens alone 23%, 12% and 8%.
+// wide kernel pays for rounds of tiles over 74 CTA pairs, which few tokens leave mostly empty, and for the gradient's
+// epilogue of the last round.  Over 120 calls (64 to 2000 tokens, 1024 to 16384 features, both directions) the choice was
+// as fast as the best of both kernels for each product, to 0.3% on average; choosing by 128, 256 and 512 tokens alone
+// was 23%, 12% and 8% slower.
 bool few_tokens(int tokens, int features, int kb, NarrowMode mode, NarrowParams& p) {
   const NarrowPlan plan = plan_narrow(mode, tokens, features, kb);
   const int64_t tiles = div_up(tokens, kGPairM) * div_up(features, mode == kNarrowProduct ? kGHalfN : kGN);
-  const double wide_us = 6.0 + (double)div_up(tiles, 74) * (0.33 * kb + 1.5);
+  const double wide_us = (mode == kNarrowProduct ? 4.0 : mode == kNarrowSlopes ? 10.0 : 6.0) + (double)div_up(tiles, 74) * (0.33 * kb + 1.5);
   p.tokens = tokens;
   p.features = features;
   p.kb = p.kb_first = kb;
