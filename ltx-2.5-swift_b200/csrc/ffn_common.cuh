@@ -37,8 +37,20 @@ __device__ __forceinline__ float activate(float g, float& slope) {
     }
     return g * s;
   } else {
-    const float s = 0.5f * erfcf(-0.70710678118654752f * g);
-    if (kSlope) slope = fmaf(g, 0.3989422804014327f * __expf(-0.5f * g * g), s);
+    // erfc(x / sqrt 2) / 2 = e^(-x^2 / 2) P(1 / (1 + 0.26 x)) for x >= 0, P of degree 7 fitted by reweighted least squares
+    // to the least relative error over [0, 14]: 3.4e-7, with what fp32 adds 6e-6 at most, of any size of the result.
+    // The slope needs the exponential too.  With erfcf in its place the first product of 101 tokens at 2048 x 5464 took
+    // 3.4 us longer where a round of tiles waits for its epilogue.
+    const float x = fabsf(g), e = __expf(-0.5f * g * g), t = __fdividef(1.0f, fmaf(0.26f, x, 1.0f));
+    float q = fmaf(t, -0.0772401318f, 0.246337339f);
+    q = fmaf(t, q, -0.135466337f);
+    q = fmaf(t, q, 0.192206472f);
+    q = fmaf(t, q, 0.0602172539f);
+    q = fmaf(t, q, 0.110970601f);
+    q = fmaf(t, q, 0.102938913f);
+    q = fmaf(t, q, 3.57263452e-05f) * e;
+    const float s = g < 0.0f ? q : 1.0f - q;
+    if (kSlope) slope = fmaf(g, 0.3989422804014327f * e, s);
     return g * s;
   }
 }

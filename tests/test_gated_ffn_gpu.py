@@ -243,6 +243,26 @@ def test_no_tokens():
     assert dx.shape == (0, 64) and all(bool((t == 0).all()) for t in dw)
 
 
+@pytest.mark.parametrize("m", [96, 6000])
+@pytest.mark.parametrize("kind", ACTS)
+def test_activations_far_out(m, kind):
+    # gate = the value, up = 1 and y = h, so y is the activation, rounded once (U, relative).  Far out on the left it is
+    # small and its exponent's error counts: arguments up to 88, three times rounded, and exp by under 2^-16 there:
+    # 2^-14 of the result together.  Below 1e-35 the exponential's own range ends.
+    gate = torch.cat((torch.linspace(-84, 84, m // 2), torch.linspace(-6, 6, m - m // 2))).cuda().bfloat16()
+    x = torch.zeros(m, 8, device="cuda", dtype=torch.bfloat16)
+    x[:, 0], x[:, 1] = gate, 1.0
+    w_gate, w_up = torch.zeros(2, 8, 8, device="cuda", dtype=torch.bfloat16)
+    w_gate[:, 0], w_up[:, 1] = 1.0, 1.0
+    w_down = torch.eye(8, device="cuda", dtype=torch.bfloat16)
+    got, kept, _ = gated_ffn(x, w_gate, w_up, w_down, kind, save=True)
+    assert torch.equal(kept, gate[:, None].expand(m, 8))
+    g = gate.double()[:, None]
+    # (1 + tanh z) / 2 as sigmoid(2 z): near -1 a float64 tanh leaves 1 + tanh an error of 2^-54, more than what is left
+    want = g * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)) if kind == "gelu_tanh" else act64(g, kind)[0]
+    assert bool(((got.double() - want).abs() <= (U + 2.0 ** -14) * want.abs() + 1e-35).all())
+
+
 @pytest.mark.parametrize("m", [3, 200])
 @pytest.mark.parametrize("kind", ACTS)
 def test_large_values_and_nan(m, kind):
