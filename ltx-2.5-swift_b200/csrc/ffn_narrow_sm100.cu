@@ -346,11 +346,11 @@ constexpr int kPlaces[kNMaxCluster + 1] = {0, 296, 296, 270, 264, 260, 264, 210,
 
 // What a cut takes, in microseconds: 1.5 a product and 3 a round of CTAs; an SM brings in 1 KB of a K slice per 10
 // ns, and 1 KB of another CTA's sums per 28 ns, and finishes a token's 128 features in 50 ns (30 for a gradient, next to
-// nothing for a plain store), for the one or two CTAs that it holds; and all weights come in at 6.4
-// TB/s, which takes the loads of 256 CTAs in flight (19 tokens at 2048 x 8192 with 128, 192 and 256 CTAs for the first
-// product: 32.3, 29.1 and 28.5 us for both).  Fitted to 2700 cuts of 128 products (96 to 1024 tokens, 1024 to 16384
-// features): the cut that it finds fastest is 0.8 us slower than the fastest one measured, on average.  The time to finish a token
-// was fitted to 70 calls by both kernels (47 to 720 tokens).
+// nothing for a plain store), for the one or two CTAs that it holds; and all weights come in at 6.4 TB/s, which takes
+// the loads of 256 CTAs in flight (19 tokens at 2048 x 8192 with 128, 192 and 256 CTAs for the first product: 32.3, 29.1
+// and 28.5 us for both).  Fitted to 2700 cuts of 128 products (96 to 1024 tokens, 1024 to 16384 features): the cut that
+// it finds fastest is 0.8 us slower than the fastest one measured, on average.  The time to finish a token was fitted to
+// 70 calls by both kernels (47 to 720 tokens).
 double cut_us(NarrowMode mode, int tokens, int features, int kb, int columns, int cluster) {
   const int parts = mode == kNarrowProduct ? 2 : 1;
   const double finish = mode == kNarrowProduct ? 0.05 : mode == kNarrowSlopes ? 0.03 : 0.0;  // of a token

@@ -64,10 +64,10 @@ constexpr int kGEpilogueWarps = 8;
 
 enum Epilogue { kProduct, kStore, kSlopes };
 
-// The epilogue's warps pass their 32 rows through shared memory, 32 columns in bf16 at a time, and TMA carries those
+// The epilogue's warps pass their 32 rows through shared memory, 32 columns in bf16 at a time or 64, and TMA carries those
 // pieces out (and the kept gate and up in): a thread finds a row in TMEM, and accesses of one row per thread take a
 // line of memory each.  A piece is 32 rows of 64 bytes in the 64-byte swizzle, which lets eight rows' threads touch all
-// banks.
+// banks; plain stores, which need no room for anything else, take 64 columns.
 constexpr uint32_t kPiece = 32 * 64;
 
 template <int kEpilogue>
@@ -75,11 +75,12 @@ struct GemmShape {
   // Pieces per warp.  Products go out through two in turn.  The gradient's epilogue has two of gate and up in turn, in
   // which dgate and dup take their place, and one of h.
   static constexpr int kPieces = kEpilogue == kSlopes ? 5 : 2;
+  static constexpr uint32_t kPieceBytes = kEpilogue == kStore ? 2 * kPiece : kPiece;  // plain stores: 64 columns
   static constexpr int kStages = kEpilogue == kSlopes ? 4 : 5;
   static constexpr uint32_t kOffPieces = kStages * kGStage;
   // full[kStages] (the first CTA's counts for both), empty[kStages], acc_full[2], acc_empty[2] (the first CTA's), and
   // two for the gate and up of each warp
-  static constexpr uint32_t kOffBar = kOffPieces + kGEpilogueWarps * kPieces * kPiece;
+  static constexpr uint32_t kOffBar = kOffPieces + kGEpilogueWarps * kPieces * kPieceBytes;
   static constexpr uint32_t kOffCtl = kOffBar + (2 * kStages + 4 + 2 * kGEpilogueWarps) * 8;  // TMEM slot, abort flag
   static constexpr uint32_t kBytes = kOffCtl + 16 + 1024;                                     // + alignment slack
   static_assert(kBytes <= kMaxDynamicSmem, "shared memory of a CTA");
@@ -184,27 +185,43 @@ __device__ __forceinline__ uint4* in_piece(uint8_t* piece, int row, int q) {
   return reinterpret_cast<uint4*>(piece + row * 64 + ((q ^ ((row >> 1) & 3)) << 4));
 }
 
-// The two pieces that a warp's products go out through, in turn.
+// The two pieces that a warp's products go out through, in turn: 32 rows (one per lane) x 32 columns, or 64 in the
+// 128-byte swizzle (all gradients of 1024 tokens at 4096 x 11008: 440 us in pieces of 32 columns, 424 in 64).  What is
+// outside the tensor is left out.
+template <int kCols>
 struct Outgoing {
   uint8_t* pieces;
   int lane;
+  uint8_t* piece = nullptr;
   int next = 0;
 
-  // 32 rows (one per lane) x 32 columns; what is outside the tensor is left out
-  __device__ __forceinline__ void send(const CUtensorMap* map, const float (&v)[32], int col, int row) {
-    uint8_t* piece = pieces + next * kPiece;
+  __device__ __forceinline__ void start() {
+    piece = pieces + next * (32 * kCols * 2);
     next ^= 1;
     if (lane == 0) piece_wait<1>();  // the one before the last has been read
     __syncwarp();
+  }
+  // 32 columns from `at` on
+  __device__ __forceinline__ void put(const float (&v)[32], int at = 0) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *in_piece(piece, lane, q) = pack8(v, 8 * q);
+    for (int q = 0; q < 4; ++q) {
+      uint4* to = kCols == 32 ? in_piece(piece, lane, q)
+                              : reinterpret_cast<uint4*>(piece + lane * 128 + (((at / 8 + q) ^ (lane & 7)) << 4));
+      *to = pack8(v, 8 * q);
+    }
+  }
+  __device__ __forceinline__ void send(const CUtensorMap* map, int col, int row) {
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
       piece_store(map, smem_u32(piece), col, row);
       bulk_commit();
     }
+  }
+  __device__ __forceinline__ void send(const CUtensorMap* map, const float (&v)[32], int col, int row) {
+    start();
+    put(v);
+    send(map, col, row);
   }
 };
 
@@ -328,8 +345,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
   } else if (warp >= 4) {
     const int quadrant = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lane_off = static_cast<uint32_t>(quadrant * 32) << 16;
-    uint8_t* pieces = sm + S::kOffPieces + (warp - 4) * S::kPieces * kPiece;
-    Outgoing outgoing{pieces, lane};
+    uint8_t* pieces = sm + S::kOffPieces + (warp - 4) * S::kPieces * S::kPieceBytes;
+    Outgoing<S::kPieceBytes / 64> outgoing{pieces, lane};
     uint64_t* kept = kept_full + 2 * (warp - 4);
     int n = 0, turn = 0;  // turn: uses of the gate and up pieces
     for (int tile = first; tile < tiles; tile += step, ++n) {
@@ -400,18 +417,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
         }
       } else if (kEpilogue == kStore) {
 #pragma unroll 1
-        for (int c = half * 128; c < half * 128 + 128; c += 32) {
+        for (int c = half * 128; c < half * 128 + 128; c += 64) {
           const int col = tn * kGN + c;
           if (col >= g.N) break;  // warp-uniform
           __syncwarp();
-          uint32_t r[32];
-          tmem_ld32(d + c, r);
+          uint32_t r[2][32];
+          tmem_ld32(d + c, r[0]);
+          tmem_ld32(d + c + 32, r[1]);
           tmem_wait_ld();
-          if (c + 32 == half * 128 + 128) release();
-          float v[32];
+          if (c + 64 == half * 128 + 128) release();
+          outgoing.start();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
-          outgoing.send(&g.out, v, col, row0);
+          for (int i = 0; i < 2; ++i) {
+            float v[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[i][e]);
+            outgoing.put(v, 32 * i);
+          }
+          outgoing.send(&g.out, col, row0);
         }
       } else {
 #pragma unroll 1
@@ -520,9 +543,10 @@ int ffn_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t
 
 namespace {
 
-// The pieces that an epilogue's warp stores and loads: boxes of 32 x 32.
-int piece_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t stride, const char* name) {
-  return ffn_map(m, ptr, rows, cols, stride, 32, name, 32);
+// The pieces that an epilogue's warp stores and loads: boxes of 32 x 32, or of 32 x 64 for plain stores.
+int piece_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t stride, const char* name,
+              int box_cols = 32) {
+  return ffn_map(m, ptr, rows, cols, stride, 32, name, box_cols);
 }
 
 // A bf16 matrix argument.
@@ -729,7 +753,7 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
   g.M = a->m;
   g.N = a->out_dim;
   g.kb = g.kb_first = kb_out;
-  if (int rc = piece_map(&g.out, a->out, a->m, a->out_dim, a->out_stride, "out")) return rc;
+  if (int rc = piece_map(&g.out, a->out, a->m, a->out_dim, a->out_stride, "out", 64)) return rc;
   return launch_gemm<false, false, kStore>(p, 1, call, st);
 }
 
@@ -849,7 +873,7 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     g.N = a->hidden;
     g.kb = 2 * kb_inner;
     g.kb_first = kb_inner;
-    if (int rc = piece_map(&g.out, a->dx, a->m, a->hidden, a->dx_stride, "dx")) return rc;
+    if (int rc = piece_map(&g.out, a->dx, a->m, a->hidden, a->dx_stride, "dx", 64)) return rc;
     if (int rc = launch_gemm<false, true, kStore>(p, 3, call, st)) return rc;
   }
   GemmParams p{};
@@ -862,7 +886,7 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     g.M = rows;
     g.N = cols;
     g.kb = g.kb_first = (int)div_up(a->m, kGK);
-    return piece_map(&g.out, out, rows, cols, out_stride, on);
+    return piece_map(&g.out, out, rows, cols, out_stride, on, 64);
   };
   if (int rc = weight(dgate, a->inner, a->inner, a->x, a->x_stride, a->hidden, a->dw_gate, a->dw_gate_stride,
                       "workspace", "x", "dw_gate"))
