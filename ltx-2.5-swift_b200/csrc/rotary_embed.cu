@@ -9,8 +9,8 @@
 // slot of a token (kP pairs, or kP elements behind the rotary part) and walks
 // over heads with cos and sin in registers.
 //
-// Angle: w reaches 1e6 radians at far positions, where fp32 keeps no fraction
-// of a turn.  The number of quarter turns is formed in fp64 and reduced there to
+// Angle: w reaches 1e6 radians at far positions, where fp32 is off by 0.03 of a
+// radian.  The number of quarter turns is formed in fp64 and reduced there to
 // [-1/2, 1/2] plus a count; only that remainder, as an angle rounded to fp32, goes
 // through sin and cos, and the quarters are sign and swap selects.  Products are
 // fp32; each element is rounded once.
