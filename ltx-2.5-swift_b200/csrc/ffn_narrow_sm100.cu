@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
     // never leave the CTA with a bulk copy still writing its shared memory
     for (int j = i < stages ? 0 : i - stages; j < i; ++j) drain_wait(full + j % stages, (j / stages) & 1);
   } else if (warp == 1 && lane == 0) {
+    grid_dep_wait();  // the limits of this kernel's waits count its own time, not that of the kernel before
     const uint32_t idesc = idesc_bf16_f32(kNRows, p.columns, kAMN, 0);
     const SDesc a0 = sdesc_split(smem_u32(sm), kAMN ? kNChunk : 16, 1024);
     const SDesc b0 = sdesc_split(smem_u32(sm) + kWeights<kMode>, 16, 1024);
@@ -202,8 +203,8 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
   // landed before an MMA that read it
   const uint32_t partial = smem_u32(sm);
   const int n_tokens = min(p.columns, p.tokens - t0);
+  grid_dep_wait();  // for these threads too, what was written before is visible, and their wait starts here
   const bool have = warp_wait(acc_full, 0, abort_flag, p.err, 67);
-  grid_dep_wait();  // over by now: for these threads too, what was written before is visible
   tc_fence_after();
   // TMEM is read 16 columns at a time: pieces start at multiples of 16, so that none reads past p.columns
   const int piece = n_tokens <= kExchange<kMode> ? kExchange<kMode> : kExchange<kMode> / 16 * 16;
