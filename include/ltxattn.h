@@ -489,6 +489,24 @@ LTXATTN_API int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* args, vo
 /* Device scratch bytes ltxattn_gated_ffn_bwd needs for these arguments. */
 LTXATTN_API size_t ltxattn_gated_ffn_bwd_workspace(const ltxattn_gated_ffn_bwd_args* args);
 
+/* How one product of the block is made. */
+typedef struct ltxattn_gated_ffn_product {
+  int32_t kernel;  /* 1: pairs of CTAs over tiles of 256 x 256; 2: tiles of 128 features for few tokens (0: no tokens) */
+  int32_t columns; /* kernel 2: tokens of a tile at most */
+  int32_t cluster; /* kernel 2: CTAs that share a tile's K */
+} ltxattn_gated_ffn_product;
+
+/* What ltxattn_gated_ffn and ltxattn_gated_ffn_bwd will launch at these sizes (introspection for benchmarks, logs and
+ * tests; host arithmetic).  The weights' gradients always take kernel 1. */
+typedef struct ltxattn_gated_ffn_plan_info {
+  ltxattn_gated_ffn_product inner;  /* x w_gate^T, x w_up^T and their product */
+  ltxattn_gated_ffn_product out;    /* its product with w_down^T */
+  ltxattn_gated_ffn_product dinner; /* dout w_down, and dgate and dup from it */
+  ltxattn_gated_ffn_product dx;     /* dgate w_gate + dup w_up */
+} ltxattn_gated_ffn_plan_info;
+LTXATTN_API int ltxattn_gated_ffn_plan(int32_t m, int32_t hidden, int32_t inner, int32_t out_dim,
+                                       ltxattn_gated_ffn_plan_info* info);
+
 /* ---- query / key preparation ---------------------------------------------- */
 
 /* Arguments of ltxattn_qk_prep: out = split-RoPE(split(rmsNorm(x, weight))).

@@ -757,6 +757,26 @@ int ltxattn_gated_ffn(const ltxattn_gated_ffn_args* a, void* stream) {
   return launch_gemm<false, false, kStore>(p, 1, call, st);
 }
 
+int ltxattn_gated_ffn_plan(int32_t m, int32_t hidden, int32_t inner, int32_t out_dim, ltxattn_gated_ffn_plan_info* info) {
+  const char* call = "ltxattn_gated_ffn_plan";
+  if (info == nullptr) return fail_ffn(LTXATTN_ERR_ARG, "%s: info is NULL", call);
+  if (int rc = check_sizes(call, LTXATTN_BF16, LTXATTN_SILU, m, hidden, inner, out_dim)) return rc;
+  *info = {};
+  if (m == 0) return LTXATTN_OK;
+  auto product = [&](NarrowMode mode, int features, int64_t k, ltxattn_gated_ffn_product* to) {
+    NarrowParams q{};
+    if (few_tokens(m, features, (int)k, mode, q))
+      *to = {2, q.columns, q.cluster};
+    else
+      *to = {1, 0, 0};
+  };
+  product(kNarrowProduct, inner, div_up(hidden, kFfnK), &info->inner);
+  product(kNarrowStore, out_dim, div_up(inner, kFfnK), &info->out);
+  product(kNarrowSlopes, inner, div_up(out_dim, kFfnK), &info->dinner);
+  product(kNarrowStoreMN, hidden, 2 * div_up(inner, kFfnK), &info->dx);
+  return LTXATTN_OK;
+}
+
 size_t ltxattn_gated_ffn_bwd_workspace(const ltxattn_gated_ffn_bwd_args* a) {
   if (a == nullptr || a->m < 1 || a->inner < 1) return 0;
   return 3 * plane_bytes(a->m, a->inner);

@@ -33,6 +33,7 @@ EXPORTED = (
     "ltxattn_out_project_workspace", "ltxattn_out_project_allreduce", "ltxattn_fwd_gather",
     "ltxattn_out_project_fused", "ltxattn_rotary_frequencies", "ltxattn_rotary_embed",
     "ltxattn_gated_ffn", "ltxattn_gated_ffn_workspace", "ltxattn_gated_ffn_bwd", "ltxattn_gated_ffn_bwd_workspace",
+    "ltxattn_gated_ffn_plan",
 )
 
 
@@ -209,6 +210,15 @@ class GatedFfnBwdArgs(ctypes.Structure):
                                   "dw_down") + _WORKSPACE
 
 
+class GatedFfnProduct(ctypes.Structure):
+    _fields_ = [("kernel", ctypes.c_int32), ("columns", ctypes.c_int32), ("cluster", ctypes.c_int32)]
+
+
+class GatedFfnPlanInfo(ctypes.Structure):
+    _fields_ = [("inner", GatedFfnProduct), ("out", GatedFfnProduct), ("dinner", GatedFfnProduct),
+                ("dx", GatedFfnProduct)]
+
+
 def load(path: str = LIB_PATH):
     """Load the in-tree library; raises when it has not been built."""
     global _lib
@@ -287,6 +297,8 @@ def load(path: str = LIB_PATH):
         getattr(L, name).restype = ctypes.c_int
         getattr(L, name + "_workspace").argtypes = [vp]
         getattr(L, name + "_workspace").restype = ctypes.c_size_t
+    L.ltxattn_gated_ffn_plan.argtypes = [ctypes.c_int32] * 4 + [ctypes.POINTER(GatedFfnPlanInfo)]
+    L.ltxattn_gated_ffn_plan.restype = ctypes.c_int
     L.ltxattn_abi_version.argtypes = []
     L.ltxattn_abi_version.restype = ctypes.c_int
     _lib = L

@@ -87,6 +87,16 @@ def _first_dim(name: str, w: torch.Tensor) -> int:
     return w.shape[0]
 
 
+def gated_ffn_plan(m: int, hidden: int, inner: int, out: int) -> dict:
+    """How the block's products are made at these sizes: for "inner", "out", "dinner" and "dx" a
+    ``(kernel, columns, cluster)`` (``ltxattn_gated_ffn_plan``; kernel 1 is the one for many tokens)."""
+    info = _lib.GatedFfnPlanInfo()
+    rc = _lib.load().ltxattn_gated_ffn_plan(m, hidden, inner, out, info)
+    if rc != _lib.OK:
+        raise Failure.from_status(rc)
+    return {n: (p.kernel, p.columns, p.cluster) for n, p in ((n, getattr(info, n)) for n, _ in info._fields_)}
+
+
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
               activation: str = "silu", save: bool = False, out: Optional[torch.Tensor] = None, stream=None):
     """x [..., hidden] -> [..., out]; w_gate and w_up [inner, hidden], w_down [out, inner] (the

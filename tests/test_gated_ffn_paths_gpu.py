@@ -1,4 +1,12 @@
-"""The gated feed-forward block on a B200: what stands before a call in its stream."""
+"""The gated feed-forward block on a B200, path by path: the kernel for many tokens in every product and with more than
+a tile to a pair of CTAs, the exchange of sums in two pieces, and what stands before a call in its stream.
+
+`forward` and `backward` of test_gated_ffn_gpu give the block in 64 bits and each tensor's bound.  Their 2^-18 for an
+activation and its slope, relative to 1 + |gate|, holds for what the kernels compute: the exponential is off by
+2 + 1.2 |x| units of 2^-24 at argument x and is multiplied by a share of at most e^x, so by under 3 units of the share's
+size 1; the fast division adds 2, the fitted polynomial of the erf form 7, the products and sums around them 4; and a
+slope is at most 1 + |gate| times as steep in the share: under 16 units, 2^-20.
+"""
 import ctypes
 import os
 import shutil
@@ -8,6 +16,7 @@ import pytest
 import torch
 
 from ltxattn import device_status, gated_ffn, gated_ffn_backward
+from test_gated_ffn_gpu import ACTS, backward, check, forward, make
 
 pytestmark = pytest.mark.gpu
 
@@ -20,11 +29,54 @@ def no_kernel_timeouts():
     assert device_status(clear=True) == 0, "a kernel wait timed out"
 
 
-def make(seed, m, hidden, inner, out, scale=1.0):
-    g = torch.Generator(device="cuda").manual_seed(seed)
-    n = lambda *s, k=1.0: (torch.randn(s, generator=g, device="cuda") * k).bfloat16()
-    return (n(m, hidden, k=scale), n(inner, hidden, k=hidden ** -0.5), n(inner, hidden, k=hidden ** -0.5),
-            n(out, inner, k=inner ** -0.5), n(m, out))
+# tokens, hidden, inner, out: test_gated_ffn_plan.py holds what they are chosen for
+WIDE = [
+    (3001, 1544, 2056, 1800),
+    (2817, 1800, 2312, 1544),  # one row past a tile, a few columns past a piece
+    (5000, 2056, 2312, 2072),  # three tiles to some pairs
+]
+# and the tokens of a tile, and the CTAs that share one
+EXCHANGE = [
+    (105, 1024, 28672, 64, 112, 1),
+    (112, 3328, 11776, 64, 112, 2),
+    (105, 1792, 9728, 64, 112, 3),
+    (112, 3840, 4608, 64, 112, 6),
+    (128, 1536, 28672, 72, 128, 1),
+    (126, 4096, 11776, 64, 128, 2),
+    (128, 2048, 9728, 64, 128, 3),
+    (113, 4096, 4608, 136, 128, 6),
+    (300, 3328, 5120, 64, 112, 2),  # the last tile's tokens fit in one piece
+]
+
+
+@pytest.mark.parametrize("kind", ACTS)
+@pytest.mark.parametrize("m,hidden,inner,out", WIDE)
+def test_many_tokens(kind, m, hidden, inner, out):
+    x, wg, wu, wd, dout = make(m + inner, m, hidden, inner, out)
+    want, want_gate, want_up = forward(x, wg, wu, wd, kind)
+    check("y", gated_ffn(x, wg, wu, wd, kind), want)
+    y, gate, up = gated_ffn(x, wg, wu, wd, kind, save=True)
+    check("y with its gate kept", y, want)
+    check("gate", gate, want_gate)
+    check("up", up, want_up)
+    got = gated_ffn_backward(x, wg, wu, wd, gate, up, dout, kind)
+    for name, g, w in zip(("dx", "dw_gate", "dw_up", "dw_down"), got, backward(x, wg, wu, wd, gate, up, dout, kind)):
+        check(name, g, w)
+    only = gated_ffn_backward(None, wg, wu, wd, gate, up, dout, kind, need_dw=False)
+    assert torch.equal(only[0], got[0])
+    only = gated_ffn_backward(x, wg, wu, wd, gate, up, dout, kind, need_dx=False)
+    assert all(torch.equal(a, b) for a, b in zip(only[1:], got[1:]))
+
+
+@pytest.mark.parametrize("m,hidden,inner,out,columns,cluster", EXCHANGE)
+def test_sums_exchanged_in_two_pieces(m, hidden, inner, out, columns, cluster):
+    x, wg, wu, wd, _ = make(m + inner, m, hidden, inner, out)
+    want, want_gate, want_up = forward(x, wg, wu, wd, "silu")
+    y, gate, up = gated_ffn(x, wg, wu, wd, save=True)
+    check("y", y, want)
+    check("gate", gate, want_gate)
+    check("up", up, want_up)
+    assert torch.equal(gated_ffn(x, wg, wu, wd), y)
 
 
 @pytest.fixture(scope="module")
