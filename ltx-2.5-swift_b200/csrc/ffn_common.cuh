@@ -15,9 +15,12 @@ namespace ltx {
 // ---------------------------------------------------------------------------
 // activations (fp32)
 
-// The fast division is off by 2 units of 2^-24, and gives 0 for a divisor above 2^126: there, for x < -87, the sigmoid
-// is below 2^-126 and 0 is as near as bf16 products need.
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+// e^-|x| never overflows, and both signs keep its relative accuracy down to where fp32 ends (with 1 / (1 + e^-x) the fast
+// division gives 0 for x < -87.3, where bf16 still holds the result).  The fast division is off by 2 units of 2^-24.
+__device__ __forceinline__ float sigmoid(float x) {
+  const float e = __expf(-fabsf(x));
+  return __fdividef(x < 0.0f ? e : 1.0f, 1.0f + e);
+}
 
 // act(g), and with kSlope its derivative too.
 template <int kAct, bool kSlope>

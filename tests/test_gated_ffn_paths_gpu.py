@@ -8,6 +8,7 @@ size 1; the fast division adds 2, the fitted polynomial of the erf form 7, the p
 slope is at most 1 + |gate| times as steep in the share: under 16 units, 2^-20.
 """
 import ctypes
+import math
 import os
 import shutil
 import subprocess
@@ -105,3 +106,42 @@ def test_a_call_behind_a_long_kernel(stays_on, m):
     assert device_status(clear=True) == 0
     assert all(torch.equal(a, b) for a, b in zip(again, (y, gate, up)))
     assert all(torch.equal(a, b) for a, b in zip(grads_again, grads))
+
+
+FAR = {"silu": (-91.5, -80.0), "gelu_tanh": (-10.0625, -9.0), "gelu": (-13.0, -11.0)}
+
+
+def far64(g, kind):
+    """The activation and its slope, without a sum of 1 and what it cancels."""
+    if kind == "gelu":
+        p = 0.5 * torch.erfc(-g / math.sqrt(2))
+        return g * p, p + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    c = 2 * math.sqrt(2 / math.pi)
+    z, dz = (g, 1.0) if kind == "silu" else (c * (g + 0.044715 * g ** 3), c * (1 + 0.134145 * g * g))
+    s = torch.sigmoid(z)
+    return g * s, s + g * s * torch.sigmoid(-z) * dz
+
+
+@pytest.mark.parametrize("kind", ACTS)
+@pytest.mark.parametrize("m,hidden,inner,out", [(96, 64, 128, 72), WIDE[0]])
+def test_activations_down_to_the_smallest_numbers(kind, m, hidden, inner, out):
+    # Results from 1e-33 down to 1.6e-38, bf16's (and fp32's) smallest with all their digits being 1.2e-38.  With up = 1
+    # and w_down the identity, y = act(gate), one rounding: 2^-8.  The exponential of arguments to 92 is off by under
+    # 112 units of 2^-24, twice that with what its argument is off in the tanh form, shares down to 1e-40 have 2^-17
+    # in fp32, and the sums and products around them a few 2^-24: under 2^-14 together.
+    gate = torch.linspace(*FAR[kind], m).cuda().bfloat16()
+    x = torch.zeros(m, hidden, device="cuda", dtype=torch.bfloat16)
+    x[:, 0], x[:, 1] = gate, 1.0
+    w_gate, w_up = torch.zeros(2, inner, hidden, device="cuda", dtype=torch.bfloat16)
+    w_gate[:, 0], w_up[:, 1] = 1.0, 1.0
+    w_down = torch.eye(out, inner, device="cuda", dtype=torch.bfloat16)
+    a, slope = far64(gate.double(), kind)
+    near = lambda got, want: bool(((got.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -14) * want.abs()).all())
+    y, kept, up = gated_ffn(x, w_gate, w_up, w_down, kind, save=True)
+    assert torch.equal(kept, gate[:, None].expand(m, inner))
+    assert near(y, a[:, None].expand(m, out))
+    # with dout = 1 for the first output alone, dx has the slope beside the gate's input and the activation beside up's
+    dout = torch.zeros(m, out, device="cuda", dtype=torch.bfloat16)
+    dout[:, 0] = 1.0
+    dx = gated_ffn_backward(x, w_gate, w_up, w_down, kept, up, dout, kind, need_dw=False)[0]
+    assert near(dx[:, 0], slope) and near(dx[:, 1], a)
