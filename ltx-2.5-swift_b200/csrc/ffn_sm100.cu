@@ -449,7 +449,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
           const bool here = warp_wait(kept + (turn & 1), (turn >> 1) & 1, abort_flag, p.err, 68);
           tmem_wait_ld();
           if (c + 32 == 128) release();
-          if (!here) continue;
+          if (!here) {
+            // another wait gave up, or this one: never leave the CTA with a copy still writing its shared memory
+            // (the next turn's is waited for in the next turn)
+            if (lane == 0) drain_wait(kept + (turn & 1), (turn >> 1) & 1);
+            continue;
+          }
           uint8_t* gp = pieces + (turn & 1) * 2 * kPiece;
           uint8_t* hp = pieces + 4 * kPiece;
           with_activation(p.activation, [&](auto act) {
