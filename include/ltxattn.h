@@ -328,8 +328,9 @@ typedef enum ltxattn_rotary_layout { LTXATTN_ROTARY_HALF = 0, LTXATTN_ROTARY_INT
  *    and divides the slowest by s (a single pair: as they are).
  *  - YARN: pairs that turn more than `fast` times in L stay, those that turn
  *    less than `slow` times are divided by s, with a linear ramp over the pair
- *    index between the two (rounded outwards to whole pairs); what is turned
- *    is multiplied by 0.1 ln(s) + 1 (1 for s <= 1).
+ *    index between the two (rounded outwards to whole pairs, from pair 0 on
+ *    at the earliest); what is turned is multiplied by 0.1 ln(s) + 1 (1 for
+ *    s <= 1).
  *  - BANDS: the same three bands with the ramp linear in the number of turns
  *    in L, and no multiplication. */
 typedef enum ltxattn_rotary_scaling {

@@ -366,8 +366,8 @@ int ltxattn_rotary_frequencies(const ltxattn_rotary_frequency_args* a, double* f
     switch (a->scaling) {
       case LTXATTN_ROTARY_LINEAR: stretched = 1; break;
       case LTXATTN_ROTARY_YARN:
-        // an empty ramp is a step just above `low`
-        stretched = std::fmin(std::fmax((j - low) / std::fmax(high - low, 0.001), 0.0), 1.0);
+        // a ramp that ends at pair 0 or before it leaves none alone; one that starts behind the last pair is never met
+        stretched = high <= 0 ? 1.0 : std::fmin(std::fmax((j - low) / std::fmax(high - low, 0.001), 0.0), 1.0);
         break;
       case LTXATTN_ROTARY_BANDS:
         stretched = 1 - std::fmin(std::fmax((a->trained_length * f / two_pi - a->slow) / (a->fast - a->slow), 0.0), 1.0);
