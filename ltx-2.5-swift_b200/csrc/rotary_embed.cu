@@ -375,6 +375,10 @@ int ltxattn_rotary_frequencies(const ltxattn_rotary_frequency_args* a, double* f
       default: break;
     }
     frequencies[j] = stretched == 0 ? f : f / a->factor * stretched + f * (1 - stretched);
+    if (!std::isfinite(frequencies[j]) || !std::isfinite(theta))
+      return fail_rotary(LTXATTN_ERR_ARG,
+                         "ltxattn_rotary_frequencies: theta (%g) with factor (%g) leaves the range of a double", a->theta,
+                         a->factor);
   }
   *magnitude =
       a->scaling == LTXATTN_ROTARY_YARN && a->factor > 1 ? (float)(0.1 * std::log(a->factor) + 1.0) : 1.0f;

@@ -14,6 +14,7 @@ to bf16, is ``apply_split_rope``.
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import Optional, Tuple
 
 import torch
@@ -39,9 +40,12 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str = "
     """
     if scaling not in SCALINGS:
         raise Failure("arg", f"scaling {scaling!r} is none of {', '.join(SCALINGS)}", _lib.ERR_ARG)
-    a = _lib.RotaryFrequencyArgs(int(rotary_dim), SCALINGS[scaling], float(theta), float(factor),
+    rotary_dim = operator.index(rotary_dim)
+    if not 0 <= rotary_dim < 2 ** 31:  # the C call's field would wrap
+        raise Failure("shape", f"rotary_dim ({rotary_dim}) must be even and >= 2, in 32 bits", _lib.ERR_SHAPE)
+    a = _lib.RotaryFrequencyArgs(rotary_dim, SCALINGS[scaling], float(theta), float(factor),
                                  float(trained_length), float(fast), float(slow))
-    out = (ctypes.c_double * max(1, int(rotary_dim) // 2))()
+    out = (ctypes.c_double * max(1, rotary_dim // 2))()
     magnitude = ctypes.c_float(1.0)
     rc = _lib.load().ltxattn_rotary_frequencies(ctypes.byref(a), out, ctypes.byref(magnitude))
     if rc != _lib.OK:

@@ -26,3 +26,28 @@ def test_yarn_keeps_the_fastest_pair_where_it_turns_at_least_once(length):
     plain, _ = table(8)
     got, _ = table(8, scaling="yarn", factor=2.0, trained_length=length)
     assert got[0] == plain[0] == 1.0 and got[-1] == plain[-1] / 2
+
+
+@pytest.mark.parametrize("kw", [
+    dict(scaling="ntk", theta=1e308, factor=8.0),      # the grown base is infinite: all pairs but the first would stand still
+    dict(scaling="linear", factor=1e-320),             # the first pair's angle is infinite
+    dict(theta=1e-320, rotary_dim=256, scaling="linear", factor=1e-5),
+])
+def test_frequencies_that_leave_the_range_are_refused(kw):
+    with pytest.raises(Failure) as e:
+        rotary_frequencies(**{"rotary_dim": 64, "device": "cpu", **kw})
+    assert e.value.kind == "arg"
+
+
+@pytest.mark.parametrize("rotary_dim", [2 ** 32 + 64, 2 ** 31, -2 ** 32 + 2, 2 ** 70])
+def test_sizes_that_are_no_32_bit_numbers_are_refused(rotary_dim):
+    # as an int32 the first is 64, the third 2; the answer must not be a table of that size
+    with pytest.raises(Failure) as e:
+        rotary_frequencies(rotary_dim, device="cpu")
+    assert e.value.kind == "shape"
+
+
+def test_a_rotary_dim_that_is_no_whole_number_is_refused():
+    for bad in (64.5, "64", None):
+        with pytest.raises((Failure, TypeError)):
+            rotary_frequencies(bad, device="cpu")
