@@ -405,7 +405,7 @@ typedef enum ltxattn_activation {
 /* Arguments of ltxattn_gated_ffn: out = (act(x w_gate^T) * (x w_up^T)) w_down^T.
  *  - x [m, hidden], w_gate and w_up [inner, hidden], w_down [out_dim, inner],
  *    out [m, out_dim]: bf16 rows of the given strides (elements), 16-byte
- *    aligned; hidden, inner and out_dim multiples of 8; any m >= 0.
+ *    aligned; hidden, inner and out_dim multiples of 8, up to 2^26; any m >= 0.
  *  - gate, up: both NULL, or [m, inner] outputs that keep x w_gate^T and
  *    x w_up^T (rounded to bf16) for the gradient.
  *  - Outputs must not overlap inputs or one another.
@@ -452,7 +452,7 @@ LTXATTN_API size_t ltxattn_gated_ffn_workspace(const ltxattn_gated_ffn_args* arg
  * [out_dim, inner] may be NULL, and is then not computed (frozen weights).
  * x is read for dw_gate and dw_up alone, w_gate and w_up for dx alone: they may
  * be NULL where those are.  Layout rules as for ltxattn_gated_ffn; with m = 0
- * the weight gradients are set to zero.  The workspace holds dgate, dup and h:
+ * the weight gradients are set to zero, and they take up to 2^27 tokens.  The workspace holds dgate, dup and h:
  * three times the forward's bytes.  Outputs must not overlap inputs or one
  * another. */
 typedef struct ltxattn_gated_ffn_bwd_args {

@@ -583,6 +583,11 @@ int check_distinct(const char* call, const Mat* mats, int count, int first) {
   return LTXATTN_OK;
 }
 
+// An epilogue waits for the whole sum of its tile, and a wait gives up after 2 s.  64 products of K take 0.33 us on every
+// row and column of a tile: with K up to 2^27 (dx: twice inner) that is 0.7 s.
+constexpr int kMaxWidth = 1 << 26;
+constexpr int kMaxSummedTokens = 1 << 27;
+
 int check_sizes(const char* call, int dtype, int activation, int m, int hidden, int inner, int out_dim) {
   if (dtype != LTXATTN_BF16) return fail_ffn(LTXATTN_ERR_DTYPE, "%s: bf16 only", call);
   if (activation < LTXATTN_SILU || activation > LTXATTN_GELU)
@@ -592,6 +597,9 @@ int check_sizes(const char* call, int dtype, int activation, int m, int hidden, 
   if (hidden % 8 || inner % 8 || out_dim % 8)
     return fail_ffn(LTXATTN_ERR_UNSUPPORTED, "%s: hidden (%d), inner (%d) and out_dim (%d) must be multiples of 8", call,
                     hidden, inner, out_dim);
+  if (std::max({hidden, inner, out_dim}) > kMaxWidth)
+    return fail_ffn(LTXATTN_ERR_UNSUPPORTED, "%s: hidden (%d), inner (%d) or out_dim (%d) is above %d", call, hidden, inner,
+                    out_dim, kMaxWidth);
   return LTXATTN_OK;
 }
 
@@ -803,6 +811,8 @@ int ltxattn_gated_ffn_bwd(const ltxattn_gated_ffn_bwd_args* a, void* stream) {
     if (int rc = check_mat(call, outs[i])) return rc;
   }
   if (!any) return LTXATTN_OK;
+  if ((dw_in || a->dw_down != nullptr) && a->m > kMaxSummedTokens)
+    return fail_ffn(LTXATTN_ERR_UNSUPPORTED, "%s: the weights' gradients of more than %d tokens", call, kMaxSummedTokens);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a->m == 0) {  // no tokens: the weights' gradients are sums of nothing
     for (int i = 1; i < 4; ++i) {
