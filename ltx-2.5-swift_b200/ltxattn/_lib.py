@@ -182,6 +182,9 @@ class RotaryEmbedArgs(ctypes.Structure):
                 ("offset", ctypes.c_int64)]
 
 
+# What packing arguments raises for a number of the wrong kind or out of its field's range.
+PACK_ERRORS = (struct.error, OverflowError, TypeError)
+
 # The bytes of a RotaryEmbedArgs, field by field (native sizes and alignment, as the C compiler lays it out): for
 # callers that pack a call's arguments at once.
 ROTARY_EMBED_ARGS = struct.Struct("@9if" + 4 * "Pqqq" + "PPiqqq")

@@ -8,6 +8,7 @@ bf16, fp32 accumulation; the product between the projections is rounded once.
 from __future__ import annotations
 
 import math
+import operator
 from typing import Optional
 
 import torch
@@ -54,6 +55,13 @@ def _output(name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor):
     return t
 
 
+def _pack(packer, *args) -> bytes:
+    try:
+        return packer.pack(*args)
+    except _lib.PACK_ERRORS as e:
+        raise Failure("arg", f"a size that the call cannot take: {e}", _lib.ERR_ARG) from None
+
+
 def _planes(n: int, m: int, inner: int, like: torch.Tensor) -> torch.Tensor:
     """A workspace of n bf16 [m, inner] planes, each rounded up to 256 bytes, as ltxattn_gated_ffn_workspace counts
     them (asking it would take another packing of the arguments).  ``like`` is bf16."""
@@ -90,6 +98,9 @@ def _first_dim(name: str, w: torch.Tensor) -> int:
 def gated_ffn_plan(m: int, hidden: int, inner: int, out: int) -> dict:
     """How the block's products are made at these sizes: for "inner", "out", "dinner" and "dx" a
     ``(kernel, columns, cluster)`` (``ltxattn_gated_ffn_plan``; kernel 1 is the one for many tokens)."""
+    for n in (m, hidden, inner, out):
+        if not -2 ** 31 <= operator.index(n) < 2 ** 31:  # the C call's arguments would wrap
+            raise Failure("shape", f"{n} is no 32-bit size", _lib.ERR_SHAPE)
     info = _lib.GatedFfnPlanInfo()
     rc = _lib.load().ltxattn_gated_ffn_plan(m, hidden, inner, out, info)
     if rc != _lib.OK:
@@ -131,7 +142,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
                 *((y.data_ptr(), out_dim) if out is None else _matrix("out", _out_rows("out", y), m, out_dim, device)),
                 *kept)
         ws = _planes(1, m, inner, x)
-        rc = _lib.load().ltxattn_gated_ffn(_lib.GATED_FFN_ARGS.pack(*args, ws.data_ptr(), 2 * ws.numel()), st)
+        rc = _lib.load().ltxattn_gated_ffn(_pack(_lib.GATED_FFN_ARGS, *args, ws.data_ptr(), 2 * ws.numel()), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
     return (y, gate, up) if save else y
@@ -182,8 +193,8 @@ def gated_ffn_backward(x: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: to
             dw_down, to[3] = _gradient("dw_down", dw_down, w_down, dout, (out_dim, inner), out_dim, inner, device)
         ws = _planes(3, m, inner, dout)
         rc = _lib.load().ltxattn_gated_ffn_bwd(
-            _lib.GATED_FFN_BWD_ARGS.pack(
-                _lib.BF16, act, m, hidden, inner, out_dim,
+            _pack(
+                _lib.GATED_FFN_BWD_ARGS, _lib.BF16, act, m, hidden, inner, out_dim,
                 *(nothing if x is None else _matrix("x", x2, m, hidden, device)),
                 *_matrix("w_gate", w_gate, inner, hidden, device), *_matrix("w_up", w_up, inner, hidden, device),
                 *_matrix("w_down", w_down, out_dim, inner, device), *_matrix("gate", gate2, m, inner, device),

@@ -143,10 +143,13 @@ def _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k
                 out_k, v_out_k = _new_like(k)
             else:
                 v_out_k = _view("out_k", out_k, k_shape, dtype, device)
-        rc = _lib.load().ltxattn_rotary_embed(
-            _lib.ROTARY_EMBED_ARGS.pack(code, B, T, H, kv_heads, D, 2 * pairs[0], order, inverse, magnitude,
-                                        q.data_ptr(), q_sb, q_sh, q_st, *v_out_q, *vk, *v_out_k,
-                                        frequencies.data_ptr(), at, bits, at_sb, at_st, offset), st)
+        try:
+            args = _lib.ROTARY_EMBED_ARGS.pack(code, B, T, H, kv_heads, D, 2 * pairs[0], order, inverse, magnitude,
+                                               q.data_ptr(), q_sb, q_sh, q_st, *v_out_q, *vk, *v_out_k,
+                                               frequencies.data_ptr(), at, bits, at_sb, at_st, offset)
+        except _lib.PACK_ERRORS as e:
+            raise Failure("arg", f"a size, offset or magnitude that the call cannot take: {e}", _lib.ERR_ARG) from None
+        rc = _lib.load().ltxattn_rotary_embed(args, st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
     return out_q if k is None else (out_q, out_k)

@@ -3,7 +3,8 @@ import ctypes
 
 import pytest
 
-from ltxattn import _lib
+from ltxattn import Failure, _lib, gated_ffn_plan
+from ltxattn.ffn import _pack
 from test_rotary_ffn_abi import bwd_args, ffn_args
 
 
@@ -31,3 +32,14 @@ def test_weight_gradients_of_too_many_tokens(only):
     assert rc == _lib.ERR_WORKSPACE, (rc, _lib.last_error())
     rc = L.ltxattn_gated_ffn_bwd(ctypes.byref(bwd_args(m=2 ** 27 + 1, **{**none, "dx": 4096 * 8, "workspace_bytes": 0})), None)
     assert rc == _lib.ERR_WORKSPACE, (rc, _lib.last_error())
+
+
+def test_sizes_past_32_bits_are_failures_of_the_call():
+    # a batch of 2^31 tokens fits on the GPU at a small width
+    many = [_lib.BF16, 0, 2 ** 31, 8, 8, 8] + 7 * [4096, 8] + [4096, 0]
+    with pytest.raises(Failure) as e:
+        _pack(_lib.GATED_FFN_ARGS, *many)
+    assert e.value.kind == "arg" and e.value.status == _lib.ERR_ARG
+    with pytest.raises(Failure) as e:
+        gated_ffn_plan(2 ** 32 + 1, 64, 64, 64)  # as an int32, one token
+    assert e.value.kind == "shape"
