@@ -50,6 +50,7 @@ def _output(name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor):
     """An output of that shape: the caller's, or a new one on the device of ``like``."""
     if t is None:
         return like.new_empty(shape) if like.dtype == torch.bfloat16 else like.new_empty(shape, dtype=torch.bfloat16)
+    _check_cuda(name, t)
     if t.shape != tuple(shape):
         raise Failure.shape(name, t.shape, str(list(shape)))
     return t
@@ -158,17 +159,22 @@ def gated_ffn_backward(x: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: to
 
     What is not needed is not computed and is None in the result: ``need_dw=False``
     for frozen weights (x may then be None), ``need_dx=False`` for a first layer.
-    The ``d...`` arguments give outputs to be written (overwritten, not added to).
+    The ``d...`` arguments give outputs to be written (overwritten, not added to); one
+    of a gradient that is not needed is refused.
     """
     act = _activation(activation)
+    for name, t, needed in (("dx", dx, need_dx), ("dw_gate", dw_gate, need_dw), ("dw_up", dw_up, need_dw),
+                            ("dw_down", dw_down, need_dw)):
+        if t is not None and not needed:
+            raise Failure("arg", f"{name} is given, but not needed", _lib.ERR_ARG)
+    if x is None and need_dw:
+        raise Failure("missing", "x is needed for the gradients of w_gate and w_up")
     _check_cuda("dout", dout)
     if dout.dim() < 1:
         raise Failure.shape("dout", dout.shape, "[..., out]")
     device = dout.get_device()
     inner = _first_dim("w_gate", w_gate)
     hidden = w_gate.shape[1]
-    if x is None and need_dw:
-        raise Failure("missing", "x is needed for the gradients of w_gate and w_up")
     lead = dout.shape[:-1]
     if len(lead) != 1:  # a matrix is checked as such below
         for name, t, cols in (("x", x, hidden), ("gate", gate, inner), ("up", up, inner)):

@@ -2,9 +2,10 @@
 import ctypes
 
 import pytest
+import torch
 
-from ltxattn import Failure, _lib, gated_ffn_plan
-from ltxattn.ffn import _pack
+from ltxattn import Failure, _lib, gated_ffn_backward, gated_ffn_plan
+from ltxattn.ffn import _output, _pack
 from test_rotary_ffn_abi import bwd_args, ffn_args
 
 
@@ -43,3 +44,18 @@ def test_sizes_past_32_bits_are_failures_of_the_call():
     with pytest.raises(Failure) as e:
         gated_ffn_plan(2 ** 32 + 1, 64, 64, 64)  # as an int32, one token
     assert e.value.kind == "shape"
+
+
+@pytest.mark.parametrize("name,kw", [("dx", dict(need_dx=False)), ("dw_gate", dict(need_dw=False)),
+                                     ("dw_up", dict(need_dw=False)), ("dw_down", dict(need_dw=False))])
+def test_outputs_of_gradients_that_are_not_needed(name, kw):
+    # they would come back as they were
+    t = torch.zeros(8, 8, dtype=torch.bfloat16)
+    with pytest.raises(Failure, match=f"{name} is given") as e:
+        gated_ffn_backward(t, t, t, t, t, t, t, **kw, **{name: t})
+    assert e.value.kind == "arg"
+
+
+def test_outputs_that_are_no_tensors():
+    with pytest.raises(Failure, match="out must be a CUDA tensor"):
+        _output("out", [0.0], (1,), torch.zeros(1))
