@@ -363,7 +363,7 @@ LTXATTN_API int ltxattn_rotary_frequencies(const ltxattn_rotary_frequency_args* 
  * of k (which may have fewer heads, as grouped-query attention has).
  *  - q, q_out: [B, heads, T, D] views; k, k_out: [B, kv_heads, T, D].  An output
  *    may be its input's own view (in place); it must not overlap an input in any
- *    other way.  Inputs may repeat rows with zero strides, outputs may not.
+ *    other way.  Inputs' rows may repeat or overlap, outputs' may not.
  *    Rows need no alignment; 16-byte aligned rows take the wide accesses.
  *  - frequencies: device array of rotary_dim / 2 doubles.
  *  - positions: device array, [B, T] with element strides (a zero stride_b

@@ -311,15 +311,15 @@ bool rows_aligned(const ltxattn_tensor& v, int64_t B, int64_t H, int64_t T, int 
 
 // Checks one input and its output; 0 or the status that fail_rotary gave.
 int check_view(const char* name, const ltxattn_tensor& x, const ltxattn_tensor& y, int64_t B, int64_t H, int64_t T,
-               int size) {
+               int D, int size) {
   if (x.data == nullptr || y.data == nullptr)
     return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_embed: %s and its output are required", name);
   if (reinterpret_cast<uintptr_t>(x.data) % size || reinterpret_cast<uintptr_t>(y.data) % size)
     return fail_rotary(LTXATTN_ERR_ALIGN, "ltxattn_rotary_embed: %s is not aligned to its type", name);
   if (x.stride_b < 0 || x.stride_h < 0 || x.stride_t < 0 || y.stride_b < 0 || y.stride_h < 0 || y.stride_t < 0)
     return fail_rotary(LTXATTN_ERR_SHAPE, "ltxattn_rotary_embed: %s has a negative stride", name);
-  if ((B > 1 && y.stride_b == 0) || (H > 1 && y.stride_h == 0) || (T > 1 && y.stride_t == 0))
-    return fail_rotary(LTXATTN_ERR_SHAPE, "ltxattn_rotary_embed: %s's output repeats rows", name);
+  if ((B > 1 && y.stride_b < D) || (H > 1 && y.stride_h < D) || (T > 1 && y.stride_t < D))
+    return fail_rotary(LTXATTN_ERR_SHAPE, "ltxattn_rotary_embed: rows of %s's output overlap", name);
   if (x.data == y.data && ((B > 1 && x.stride_b != y.stride_b) || (H > 1 && x.stride_h != y.stride_h) ||
                            (T > 1 && x.stride_t != y.stride_t)))
     return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_embed: %s in place needs the input's own strides", name);
@@ -416,9 +416,9 @@ int ltxattn_rotary_embed(const ltxattn_rotary_embed_args* a, void* stream) {
   const bool bf16 = a->dtype == LTXATTN_BF16;
   const int size = bf16 ? 2 : 4;
   if (H > 0)
-    if (int rc = check_view("q", a->q, a->q_out, B, H, T, size)) return rc;
+    if (int rc = check_view("q", a->q, a->q_out, B, H, T, a->head_dim, size)) return rc;
   if (Hk > 0)
-    if (int rc = check_view("k", a->k, a->k_out, B, Hk, T, size)) return rc;
+    if (int rc = check_view("k", a->k, a->k_out, B, Hk, T, a->head_dim, size)) return rc;
 
   if (H > 0 && Hk > 0 && (a->q_out.data == a->k_out.data || a->q_out.data == a->k.data || a->k_out.data == a->q.data))
     return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_embed: an output of q or k is the other's memory");
