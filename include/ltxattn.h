@@ -369,6 +369,7 @@ LTXATTN_API int ltxattn_rotary_frequencies(const ltxattn_rotary_frequency_args* 
  *  - positions: device array, [B, T] with element strides (a zero stride_b
  *    shares one row), int64 or int32 (position_bits 64 or 32), any sign; NULL:
  *    token t stands at t.  `offset` is added to each position.
+ *  - magnitude: finite.
  *  - inverse: turn the other way; with the same magnitude this is the gradient
  *    (the transpose) of the call without it.
  * Angles are formed and reduced to an eighth of a turn in fp64 (position + offset

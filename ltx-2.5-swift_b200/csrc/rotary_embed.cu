@@ -398,6 +398,8 @@ int ltxattn_rotary_embed(const ltxattn_rotary_embed_args* a, void* stream) {
                        a->rotary_dim, a->head_dim);
   if (a->layout != LTXATTN_ROTARY_HALF && a->layout != LTXATTN_ROTARY_INTERLEAVED)
     return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_embed: unknown layout %d", a->layout);
+  if (!std::isfinite(a->magnitude))
+    return fail_rotary(LTXATTN_ERR_ARG, "ltxattn_rotary_embed: magnitude (%g) must be finite in fp32", a->magnitude);
   if (a->positions != nullptr && a->position_bits != 64 && a->position_bits != 32)
     return fail_rotary(LTXATTN_ERR_DTYPE, "ltxattn_rotary_embed: positions must be 64- or 32-bit integers");
   const int64_t B = a->batch, T = a->tokens, H = a->heads, Hk = a->kv_heads;

@@ -15,3 +15,11 @@ def test_outputs_whose_rows_overlap(kw):
     rc = _lib.load().ltxattn_rotary_embed(ctypes.byref(rotary_args(**kw)), None)
     assert rc == _lib.ERR_SHAPE, (rc, _lib.last_error())
     assert "overlap" in _lib.last_error()
+
+
+@pytest.mark.parametrize("magnitude", [float("inf"), float("-inf"), float("nan"), 1e39])
+def test_magnitudes_that_are_not_finite(magnitude):
+    # 1e39 is infinite in the call's fp32
+    a = rotary_args(magnitude=magnitude)
+    assert _lib.load().ltxattn_rotary_embed(ctypes.byref(a), None) == _lib.ERR_ARG
+    assert "magnitude" in _lib.last_error()
