@@ -166,6 +166,12 @@ class _on:
         return False
 
 
+def _written(outputs) -> None:
+    """Tells autograd that the caller's tensors were written, so that a graph that kept one of them says so instead of
+    taking its new contents."""
+    torch.autograd.graph.increment_version(outputs)
+
+
 class AttentionBackend:
     """The attention seam, backed by libltxattn_cuda."""
 

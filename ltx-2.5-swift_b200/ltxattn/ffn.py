@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .backend import Failure, _check_cuda, _on
+from .backend import Failure, _check_cuda, _on, _written
 
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1, "gelu": 2}
 
@@ -117,7 +117,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     ``activation`` is "silu", "gelu_tanh" or "gelu" (erf).  With ``save`` the result
     is ``(y, gate, up)``, the last two being what ``gated_ffn_backward`` needs:
     ``x w_gate^T`` and ``x w_up^T``, [..., inner].  hidden, inner and out are
-    multiples of 8 and rows 16-byte aligned.
+    multiples of 8 and rows 16-byte aligned.  Results carry no graph.
     """
     act = _activation(activation)
     _check_cuda("x", x)
@@ -146,6 +146,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         rc = _lib.load().ltxattn_gated_ffn(_pack(_lib.GATED_FFN_ARGS, *args, ws.data_ptr(), 2 * ws.numel()), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
+    if out is not None:
+        _written([out])
     return (y, gate, up) if save else y
 
 
@@ -182,6 +184,7 @@ def gated_ffn_backward(x: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: to
                 _check_cuda(name, t)
                 if t.shape != lead + (cols,):
                     raise Failure.shape(name, t.shape, str(list(lead) + [cols]))
+    given = [t for t in (dx, dw_gate, dw_up, dw_down) if t is not None]
     with _on(device, stream) as st:
         if len(lead) == 1:
             d2, x2, gate2, up2 = dout, x, gate, up
@@ -208,4 +211,6 @@ def gated_ffn_backward(x: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: to
                 *to[2], *to[3], ws.data_ptr(), 2 * ws.numel()), st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
+    if given:
+        _written(given)
     return (dx if need_dx else None,) + ((dw_gate, dw_up, dw_down) if need_dw else (None, None, None))

@@ -20,7 +20,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .backend import Failure, _check_cuda, _dtype_code, _on
+from .backend import Failure, _check_cuda, _dtype_code, _on, _written
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
@@ -133,6 +133,7 @@ def _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k
         at, at_st = positions.data_ptr(), strides[-1]
         if len(at_shape) == 2 and at_shape[0] > 1:
             at_sb = strides[0]
+    given = [t for t in (out_q, out_k) if t is not None]
     with _on(device, stream) as st:
         if out_q is None:
             out_q, v_out_q = _new_like(q)
@@ -152,6 +153,8 @@ def _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k
         rc = _lib.load().ltxattn_rotary_embed(args, st)
     if rc != _lib.OK:
         raise Failure.from_status(rc)
+    if given:
+        _written(given)
     return out_q if k is None else (out_q, out_k)
 
 
@@ -167,6 +170,7 @@ def rotary_embed(q: torch.Tensor, frequencies: torch.Tensor, k: Optional[torch.T
     its cache).  ``layout`` "half" turns element j with j + rotaryDim / 2,
     "interleaved" 2j with 2j + 1.  Angles are formed in fp64, each element is
     rounded once.  Outputs may be the inputs themselves, or a cache's slots.
+    Results carry no graph: gradients are ``rotary_embed_backward``'s.
     Returns the turned q, or (q, k).
     """
     return _embed(q, frequencies, k, positions, offset, layout, magnitude, out_q, out_k, stream, 0)

@@ -145,3 +145,15 @@ def test_activations_down_to_the_smallest_numbers(kind, m, hidden, inner, out):
     dout[:, 0] = 1.0
     dx = gated_ffn_backward(x, w_gate, w_up, w_down, kept, up, dout, kind, need_dw=False)[0]
     assert near(dx[:, 0], slope) and near(dx[:, 1], a)
+
+
+def test_outputs_given_by_the_caller_count_as_written():
+    x, wg, wu, wd, dout = make(32, 5, 64, 128, 72)
+    _, gate, up = gated_ffn(x, wg, wu, wd, save=True)
+    out, dx, dwg, dwu, dwd = (torch.empty_like(t) for t in (dout, x, wg, wu, wd))
+    inputs = (x, wg, wu, wd, gate, up, dout)
+    before = [t._version for t in inputs]
+    gated_ffn(x, wg, wu, wd, out=out)
+    gated_ffn_backward(x, wg, wu, wd, gate, up, dout, dx=dx, dw_gate=dwg, dw_up=dwu, dw_down=dwd)
+    assert all(t._version > 0 for t in (out, dx, dwg, dwu, dwd))
+    assert [t._version for t in inputs] == before
