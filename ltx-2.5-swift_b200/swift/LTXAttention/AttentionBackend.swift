@@ -251,7 +251,11 @@ public enum AttentionBackend {
         a.inverse = inverse ? 1 : 0
         a.magnitude = magnitude
         a.q = q.c; a.q_out = qOut.c
-        if let k, let kOut { a.kv_heads = kvHeads; a.k = k.c; a.k_out = kOut.c }
+        if k != nil || kOut != nil {  // one without the other is refused by the call
+            a.kv_heads = kvHeads
+            if let k { a.k = k.c }
+            if let kOut { a.k_out = kOut.c }
+        }
         a.frequencies = frequencies
         a.positions = UnsafeRawPointer(positions); a.position_bits = 64
         a.position_stride_b = positionStrides.b; a.position_stride_t = positionStrides.t
