@@ -89,7 +89,7 @@ struct GemmShape {
 // One output of a launch (a launch of the weight gradients has up to three).
 struct Gemm {
   CUtensorMap a[2], b[2];  // K slices beyond kb_first come from the second pair
-  CUtensorMap out;         // in pieces of 32 x 32
+  CUtensorMap out;         // in pieces of 32 x 32, plain stores of 32 x 64
   int M, N;                // rows and accumulator columns that exist (kProduct: columns of h)
   int kb, kb_first;        // 64-wide K slices in all, and those of the first pair
   int tiles_m, tiles_n;
@@ -655,7 +655,7 @@ int launch_gemm(GemmParams& p, int slot, const char* call, cudaStream_t st) {
 }
 
 // Whether a product runs feature by feature (ffn_narrow_sm100.cu), by what both kernels were measured to take.  The
-// wide kernel pays for rounds of tiles over 74 CTA pairs, which few tokens leave mostly empty, and for the gradient's
+// wide kernel pays for rounds of tiles over 74 CTA pairs (148 SMs), which few tokens leave mostly empty, and for the gradient's
 // epilogue of the last round.  Over 120 calls (64 to 2000 tokens, 1024 to 16384 features, both directions) the choice was
 // as fast as the best of both kernels for each product, to 0.3% on average; choosing by 128, 256 and 512 tokens alone
 // was 23%, 12% and 8% slower.

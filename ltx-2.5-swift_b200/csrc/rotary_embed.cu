@@ -117,7 +117,8 @@ __device__ __forceinline__ void from_f(__nv_bfloat16& d, float v) { d = __float2
 // cos and sin of position * frequency (see the head of the file).  The number of
 // quarter turns is rounded by adding 1.5 * 2^52, which leaves it in the low bits
 // of the sum (for angles below 2^51 quarters).  The remainder is at most pi / 4,
-// where the Taylor series to x^9 and x^10 are within 2^-29 of sin x / x and cos x.
+// where the Taylor series to x^9 and x^10 are within 2^-28.5 of sin x and 2^-32 of
+// cos x, relative to them; fp32 adds some 2^-23.
 __device__ __forceinline__ void turn(double position, double frequency, float& c, float& s) {
   constexpr double kMagic = 6755399441055744.0, kQuarter = 1.57079632679489661923;
   const double quarters = position * frequency * 0.63661977236758134308;  // 2 / pi
@@ -211,9 +212,9 @@ struct Slot {
 // by gridDim.y CTAs, each making the cos and sin again).  The heads of a token lie side by
 // side in a projection's output, so a CTA streams whole rows of it.  Many small
 // CTAs keep the memory busy better than more runs per thread: 128 threads at 48
-// registers take 150 us for 29760 tokens x 64 heads x 128 in bf16 (6.5 TB/s, 0.99
-// of the measured copy); fetching a head ahead of the one that turns 158, four
-// heads at once 257.
+// registers (for which seven of the instances spill 4 to 36 bytes) take 150 us for
+// 29760 tokens x 64 heads x 128 in bf16 (6.5 TB/s, 0.99 of the measured copy);
+// fetching a head ahead of the one that turns 158, four heads at once 257.
 template <typename T, int kP, bool kInterleaved>
 __global__ void __launch_bounds__(kRThreads, 5) rotary_embed_kernel(const __grid_constant__ RotaryEmbedParams p) {
   extern __shared__ float2 turns[];  // [token_lanes][pairs]: (cos, sin), with the magnitude
@@ -465,7 +466,7 @@ int ltxattn_rotary_embed(const ltxattn_rotary_embed_args* a, void* stream) {
   p.head_lanes = std::max(1, std::min((int)std::max(H, Hk), kTargetThreads / p.slot_lanes));
   const int64_t items = int64_t(p.rows) * p.slots;
   p.few_heads = H + Hk <= kFewHeads && items >= 148 * 1024 && items <= 0x7fffffff - kRThreads;
-  // few tokens: as many CTAs to a token as fill the GPU, at a head to a thread at least
+  // few tokens: as many CTAs to a token as fill the GPU (148 SMs), at a head to a thread at least
   const int64_t threads = std::min<int64_t>(int64_t(p.rows) * p.slot_lanes * p.head_lanes, 148 * 1024);
   p.head_groups = (int)std::min<int64_t>({148 * 1024 / threads, (std::max(H, Hk) + p.head_lanes - 1) / p.head_lanes, 65535});
   p.token_lanes = std::max(1, kTargetThreads / (p.slot_lanes * p.head_lanes));
