@@ -157,3 +157,80 @@ def test_outputs_given_by_the_caller_count_as_written():
     gated_ffn_backward(x, wg, wu, wd, gate, up, dout, dx=dx, dw_gate=dwg, dw_up=dwu, dw_down=dwd)
     assert all(t._version > 0 for t in (out, dx, dwg, dwu, dwd))
     assert [t._version for t in inputs] == before
+
+
+@pytest.mark.parametrize("m", [3, 100])
+def test_weights_that_the_call_before_wrote(m):
+    # The second product of a call loads its weights before the first is complete; what wrote them may be the call
+    # before.  Outputs of one call are the next one's weights, each in turn, with nothing between the calls.
+    hidden, inner, out = 256, 1024, 512
+    x, wg, wu, wd, dout = make(33, m, hidden, inner, out)
+    makers = {"w_gate": make(34, inner, 2048, 4096, hidden)[:4], "w_up": make(35, inner, 2048, 4096, hidden)[:4],
+              "w_down": make(36, out, 2048, 4096, inner)[:4]}
+    base = {"w_gate": wg, "w_up": wu, "w_down": wd}
+    _, gate, up = gated_ffn(x, wg, wu, wd, save=True)
+    for name, maker in makers.items():
+        new = gated_ffn(*maker)
+        torch.cuda.synchronize()
+        weights = {**base, name: new}
+        want = gated_ffn(x, **weights)
+        want_dx = gated_ffn_backward(None, **weights, gate=gate, up=up, dout=dout, need_dw=False)[0]
+        for _ in range(3):
+            buf = torch.full_like(new, float("nan"))
+            torch.cuda.synchronize()
+            gated_ffn(*maker, out=buf)
+            assert torch.equal(gated_ffn(x, **{**base, name: buf}), want), name
+            buf.fill_(float("nan"))
+            torch.cuda.synchronize()
+            gated_ffn(*maker, out=buf)
+            dx = gated_ffn_backward(None, **{**base, name: buf}, gate=gate, up=up, dout=dout, need_dw=False)[0]
+            assert torch.equal(dx, want_dx), name
+
+
+@pytest.mark.parametrize("kind", ACTS)
+@pytest.mark.parametrize("m,hidden,inner,out", [(20, 64, 136, 72), WIDE[0]])
+def test_infinite_tokens(kind, m, hidden, inner, out):
+    # positive weights: an infinite input makes gate and up infinite, the activation of the one keeps its sign, and the
+    # output is infinite with it; other tokens do not see it
+    x, wg, wu, wd, dout = make(37, m, hidden, inner, out)
+    wg, wu, wd = wg.abs() + 2.0 ** -9, wu.abs() + 2.0 ** -9, wd.abs() + 2.0 ** -9
+    y, gate, up = gated_ffn(x, wg, wu, wd, kind, save=True)
+    spoiled = x.clone()
+    spoiled[1, 5] = float("inf")
+    z, zgate, zup = gated_ffn(spoiled, wg, wu, wd, kind, save=True)
+    rest = torch.arange(m, device="cuda") != 1
+    assert bool((zgate[1] == float("inf")).all()) and bool((zup[1] == float("inf")).all())
+    assert bool((z[1] == float("inf")).all()) and torch.equal(z[rest], y[rest])
+    # an infinite gradient spoils its own token's dx, and the weights' gradients as sums over tokens
+    dx = gated_ffn_backward(None, wg, wu, wd, gate, up, dout, kind, need_dw=False)[0]
+    dout[2, 3] = float("inf")
+    got = gated_ffn_backward(x, wg, wu, wd, gate, up, dout, kind)
+    keep = torch.arange(m, device="cuda") != 2
+    assert torch.equal(got[0][keep], dx[keep]) and not bool(got[0][2].isfinite().any())
+    others = torch.arange(out, device="cuda") != 3
+    assert bool(got[3][others].isfinite().all()) and not bool(got[3][3].isfinite().any())
+
+
+def test_tokens_of_any_rank():
+    x, wg, wu, wd, dout = make(38, 12, 64, 128, 72)
+    y, gate, up = gated_ffn(x, wg, wu, wd, save=True)
+    grads = gated_ffn_backward(x, wg, wu, wd, gate, up, dout)
+    # one token without a leading dim
+    one, g1, u1 = gated_ffn(x[4], wg, wu, wd, save=True)
+    want1 = gated_ffn(x[4:5], wg, wu, wd, save=True)
+    assert all(a.dim() == 1 and torch.equal(a, b[0]) for a, b in zip((one, g1, u1), want1))
+    got1 = gated_ffn_backward(x[4], wg, wu, wd, g1, u1, dout[4])
+    want1 = gated_ffn_backward(x[4:5], wg, wu, wd, want1[1], want1[2], dout[4:5])
+    assert got1[0].shape == (64,) and torch.equal(got1[0], want1[0][0])
+    assert all(torch.equal(a, b) for a, b in zip(got1[1:], want1[1:]))
+    # leading dims that do not collapse into rows are copied, on the call's own stream
+    t4 = lambda t: t.view(2, 3, 2, -1).transpose(1, 2).contiguous().transpose(1, 2)
+    side = torch.cuda.Stream()
+    x4, gate4, up4, dout4 = t4(x), t4(gate), t4(up), t4(dout)
+    torch.cuda.synchronize()
+    y4 = gated_ffn(x4, wg, wu, wd, stream=side)
+    got4 = gated_ffn_backward(x4, wg, wu, wd, gate4, up4, dout4, stream=side)
+    torch.cuda.synchronize()
+    assert y4.shape == (2, 3, 2, 72) and torch.equal(y4.reshape(12, 72), y)
+    assert got4[0].shape == (2, 3, 2, 64) and torch.equal(got4[0].reshape(12, 64), grads[0])
+    assert all(torch.equal(a, b) for a, b in zip(got4[1:], grads[1:]))

@@ -1,4 +1,6 @@
 """Calls of the rotary entry points on a B200 that their documentation allows, or that they must refuse."""
+import math
+
 import pytest
 import torch
 
@@ -34,3 +36,37 @@ def test_a_graph_that_kept_what_is_turned_in_place_says_so():
     with torch.inference_mode():
         t = torch.zeros(1, 2, 3, 64, device="cuda")
         rotary_embed(t, freq, out_q=t)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_infinities_stay_in_their_pair(layout, dtype):
+    g = torch.Generator(device="cuda").manual_seed(41)
+    x = torch.randn((2, 3, 7, 64), generator=g, device="cuda").to(dtype)
+    freq, _ = rotary_frequencies(48)
+    y = rotary_embed(x, freq, layout=layout, offset=3)
+    a, b = (5, 5 + 24) if layout == "half" else (10, 11)
+    x[0, 1, 4, a], x[1, 2, 6, 60] = float("inf"), float("-inf")  # one that is turned and one that is copied
+    z = rotary_embed(x, freq, layout=layout, offset=3)
+    same = torch.ones_like(x, dtype=torch.bool)
+    same[0, 1, 4, a] = same[0, 1, 4, b] = same[1, 2, 6, 60] = False
+    assert torch.equal(z[same], y[same])
+    angle = 7 * freq[5].cpu()
+    assert z[0, 1, 4, a].item() == math.copysign(math.inf, angle.cos().item())
+    assert z[0, 1, 4, b].item() == math.copysign(math.inf, angle.sin().item())
+    assert z[1, 2, 6, 60].item() == -math.inf
+
+
+def test_turned_keys_feed_the_next_call():
+    # calls in a row on one stream, each reading what the one before wrote: n turns by 1 are one by n
+    g = torch.Generator(device="cuda").manual_seed(42)
+    x = torch.randn((1, 8, 500, 128), generator=g, device="cuda")
+    freq, _ = rotary_frequencies(128)
+    ones = torch.ones(500, dtype=torch.int64, device="cuda")
+    y = x
+    for _ in range(20):
+        y = rotary_embed(y, freq, positions=ones)
+    want = rotary_embed(x, freq, positions=20 * ones)
+    # each of 21 turns is off by under 2^-21 + 2^-24 of the pair's size, and a pair keeps its size
+    size = x[..., :64].hypot(x[..., 64:]).repeat(1, 1, 1, 2)
+    assert bool(((y - want).abs() <= 21 * 1.5 * (2.0 ** -21 + 2.0 ** -24) * size).all())
