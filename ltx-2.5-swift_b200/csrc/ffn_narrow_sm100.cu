@@ -13,7 +13,9 @@
 // tile: each takes a part of K, leaves its fp32 partial in its own shared
 // memory, and after a cluster barrier the CTAs add the parts of a share of the
 // tokens each, in rank order, and finish those (the sums do not depend on which
-// CTA came first).
+// CTA came first).  Roundings are those of ffn_sm100.cu: sums are exchanged and
+// finished in fp32; h, dgate and dup are rounded to bf16 once, as operands of the
+// next product.
 //
 // The kernel that follows another (the second product of a call) starts while
 // that one ends: its weights do not depend on it, so the first stages are loaded

@@ -35,8 +35,9 @@
 // (1.48 PFLOP/s, 0.89 of the measured burst rate of a library GEMM) and 976 back
 // to back under the power cap (0.93 of the measured sustained rate; the two bare
 // products in the library: 802 and 942).  The backward takes 1829 and 2100 us
-// (library products alone: 1619 and 1898); the difference is dh's epilogue, whose
-// 640 KB a tile share the shared-memory bandwidth that the MMAs nearly fill.
+// (library products alone: 1619 and 1898); the difference is mostly dh's epilogue,
+// which moves 640 KB through shared memory a tile and keeps the tensor pipe to 65%
+// of its launch, where the other products' is busy for 88%.
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
