@@ -70,3 +70,27 @@ def test_turned_keys_feed_the_next_call():
     # each of 21 turns is off by under 2^-21 + 2^-24 of the pair's size, and a pair keeps its size
     size = x[..., :64].hypot(x[..., 64:]).repeat(1, 1, 1, 2)
     assert bool(((y - want).abs() <= 21 * 1.5 * (2.0 ** -21 + 2.0 ** -24) * size).all())
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("heads", [3, 40])  # a thread through all heads of a token, and tokens with their own CTAs
+@pytest.mark.parametrize("call,sign", [(rotary_embed, 1.0), (rotary_embed_backward, -1.0)])
+def test_turns_to_the_accuracy_of_fp32(call, sign, layout, heads):
+    # The bound from what the kernel computes, u = 2^-24.  Angles up to 1e6 radians are off by under 2^-31 in fp64, here
+    # and in the kernel; the remainder, under pi / 4, is rounded to fp32: u / 2.  The sine's series leaves 2^-29; its last
+    # sum rounds by u / 2, and its term x^3 ps, under 0.081, is off by 5 u of itself: 0.95 u + 2^-29 together.  The cosine's
+    # x^2 pc, under 0.31, is off by 2.5 u of itself, and its sum rounds by u / 2: 1.3 u + 2^-32.  So (cos, sin) are off by
+    # 1.8 u and 1.5 u; b sin is rounded by u, and the sum once, relative to it: 2.5 u (|a| + |b|) + u |out| holds both.
+    g = torch.Generator(device="cuda").manual_seed(43)
+    D, T = 128, 25000 if heads == 3 else 900
+    x = torch.randn((1, heads, T, D), generator=g, device="cuda")
+    place = torch.randint(0, 1000000, (T,), generator=g, device="cuda")
+    freq, _ = rotary_frequencies(D)
+    got = call(x, freq, positions=place, layout=layout).double()
+    angle = sign * place.double()[:, None] * freq
+    cos, sin = angle.cos(), angle.sin()
+    pair = (lambda t: (t[..., :D // 2], t[..., D // 2:])) if layout == "half" else (lambda t: (t[..., 0::2], t[..., 1::2]))
+    a, b = pair(x.double())
+    u = 2.0 ** -24
+    for out, want in zip(pair(got), (a * cos - b * sin, b * cos + a * sin)):
+        assert bool(((out - want).abs() <= 2.5 * u * (a.abs() + b.abs()) + u * want.abs()).all())
