@@ -121,8 +121,10 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// The same without an order on memory.
-__device__ __forceinline__ void cluster_barrier_relaxed() {
+// The same for CTAs that have read one another's shared memory and write nothing that another reads: the fence ends
+// the reads before the arrival, without waiting for stores on their way to global memory.
+__device__ __forceinline__ void cluster_barrier_after_reads() {
+  asm volatile("fence.acq_rel.cta;" ::: "memory");
   asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   asm volatile("barrier.cluster.wait;" ::: "memory");
 }

@@ -274,12 +274,12 @@ __global__ void __launch_bounds__(kNThreads, 2) narrow_kernel(const __grid_const
         store4(p.out + token * p.out_stride + col, v);
       }
     }
-    // No CTA writes the next tokens' sums, or leaves, while another reads these.  To leave takes no order on memory (what
-    // a thread has read it has used by now), and without one nothing waits for the stores: 1 us a product.
+    // No CTA writes the next tokens' sums, or leaves, while another reads these.  To leave takes no order on what was
+    // written, and without one nothing waits for the stores: 1 us a product.
     if (c0 + piece < n_tokens)
       cluster_barrier();
     else
-      cluster_barrier_relaxed();
+      cluster_barrier_after_reads();
   }
   tc_fence_before();
   __syncthreads();
